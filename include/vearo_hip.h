@@ -427,6 +427,89 @@ int vh_fused_attention_bwd_probs(const float* P, const float* q, const vh_layout
                                  const vh_layout* dkl, float* dv, const vh_layout* dvl,
                                  void* scratch, size_t scratch_bytes, void* stream);
 
+/* ------------------------------------------- packed training: from projection to loss -- */
+
+/* Operators of training on packed batches: T tokens that hold several sequences one
+ * behind the other, with no padding between them. No counterpart in the reference, whose
+ * batches are padded [B, S] blocks; they stand beside the layernorm, fused attention and
+ * cross-entropy entries above and follow their rules. Layouts here are rank 3, [T, H, D]:
+ * tokens, heads, head size; any strides, unit stride on D (a column block of one
+ * projection is such a layout). Outputs may not overlap an input except where said.
+ * Called with scratch NULL the library takes it from the arena; on a stream under graph
+ * capture the caller must pass it (VH_ERR_INVALID otherwise), and graphs that may run at
+ * once need one each. */
+
+/* Queries and keys normed per head and rotated by their token's position, in one pass:
+ *   u = x / sqrt(mean(x^2) + eps) * w over each head's D elements, then the first
+ *   `rotary` elements turned in pairs by the angle positions[t] * base^(-2i/rotary):
+ *   pair i is elements (i, i + rotary/2), or (2i, 2i + 1) where interleaved != 0.
+ * q, qo: [T, Hq, D]; k, ko: [T, Hk, D]; wq, wk: [D]; positions: [T] f32 (any real
+ * numbers; the angles are formed in 64 bits). 0 <= rotary <= D, even; D <= 256;
+ * base > 0, eps >= 0. qo may be q and ko k in the same layout. */
+int vh_qk_norm_rope_fwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
+                        const float* wk, const float* positions, float eps, double base, int32_t rotary,
+                        int32_t interleaved, float* qo, const vh_layout* qol, float* ko, const vh_layout* kol,
+                        void* stream);
+/* Its backward from the same inputs and the results' gradients dqo, dko: dq, dk, and the
+ * weights' gradients dwq[D], dwk[D], summed over tokens and heads in a fixed order (no
+ * atomics). dq may be dqo or q, and dk dko or k, in the same layout. scratch: NULL or
+ * vh_qk_norm_rope_bwd_scratch_bytes(T, D) bytes. */
+int vh_qk_norm_rope_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
+                        const float* wk, const float* positions, float eps, double base, int32_t rotary,
+                        int32_t interleaved, const float* dqo, const vh_layout* dqol, const float* dko,
+                        const vh_layout* dkol, float* dq, const vh_layout* dql, float* dk, const vh_layout* dkl,
+                        float* dwq, float* dwk, void* scratch, size_t scratch_bytes, void* stream);
+size_t vh_qk_norm_rope_bwd_scratch_bytes(int64_t T, int64_t D);
+
+/* Attention within each of n packed sequences, with grouped heads: q, out: [T, Hq, D];
+ * k, v: [T, Hk, D]; query head h reads key head h / (Hq / Hk); Hq a multiple of Hk,
+ * D <= 256. starts: n + 1 int32 in device memory, not decreasing, in [0, T]: sequence s
+ * is tokens starts[s] .. starts[s + 1] - 1 (it may be empty); tokens in no sequence are
+ * not read, and their rows of every output are left as they were. With causal != 0 a
+ * query sees the keys up to its own token, else its whole sequence; what a query does not
+ * see does not reach its row, infinities and NaN included. scale > 0 multiplies the
+ * scores. lse: [Hq, T], each row's log of the sum of exp of its scores, kept for the
+ * backward. Scores are never stored. A starts array that breaks its rule computes nothing
+ * and raises VH_ERR_DEVICE_PANIC at the next vh_sync.
+ * scratch: NULL or vh_packed_attention_scratch_bytes(T, n, Hq, Hk, D, 0) bytes. */
+int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
+                            const vh_layout* vl, const int32_t* starts, int64_t n, float scale, int causal, float* out,
+                            const vh_layout* ol, float* lse, void* scratch, size_t scratch_bytes, void* stream);
+/* dq [T, Hq, D], dk and dv [T, Hk, D] from the forward's inputs, its out and lse, and
+ * dout [T, Hq, D]. Every sum in a fixed order (no atomics): the same bits each time.
+ * scratch: NULL or vh_packed_attention_scratch_bytes(T, n, Hq, Hk, D, 1) bytes. */
+int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
+                            const vh_layout* vl, const int32_t* starts, int64_t n, float scale, int causal,
+                            const float* out, const vh_layout* ol, const float* lse, const float* dout,
+                            const vh_layout* dol, float* dq, const vh_layout* dql, float* dk, const vh_layout* dkl,
+                            float* dv, const vh_layout* dvl, void* scratch, size_t scratch_bytes, void* stream);
+size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D, int backward);
+
+/* loss[0] = mean over the counted rows r of -log_softmax(x[r] w^T)[targets[r]], without
+ * keeping the [R, V] logits: they are formed in pieces of rows, in scratch. x: R rows of D,
+ * ldx floats apart; w: V rows of D, ldw apart; targets: [R] f32 class ids as above, a row
+ * whose target equals `ignore` not counted (NaN: none is). No counted row: loss 0.
+ * row_stats: [R, 2], each row's max logit and sum of exp(logit - max), kept for the
+ * backward (8-byte aligned). scratch: NULL or
+ * vh_linear_cross_entropy_scratch_bytes(R, V) bytes. Not under graph capture
+ * (VH_ERR_UNSUPPORTED: the products inside take workspaces of their own). */
+int vh_linear_cross_entropy_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                float ignore, float* loss, float* row_stats, int64_t R, int64_t D, int64_t V,
+                                void* scratch, size_t scratch_bytes, void* stream);
+/* dx [R, D] and dw [V, D] (row strides lddx, lddw), written in full, from those
+ * statistics and the device scalar grad_out[0]; the logits are formed again. */
+int vh_linear_cross_entropy_bwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                float ignore, const float* row_stats, const float* grad_out, float* dx, int64_t lddx,
+                                float* dw, int64_t lddw, int64_t R, int64_t D, int64_t V, void* scratch,
+                                size_t scratch_bytes, void* stream);
+/* Both in one call that forms the logits once, for a loss whose gradient is known
+ * beforehand (the graph's root, as vh_cross_entropy_fwd_bwd_ld). */
+int vh_linear_cross_entropy_fwd_bwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                    float ignore, const float* grad_out, float* loss, float* dx, int64_t lddx,
+                                    float* dw, int64_t lddw, int64_t R, int64_t D, int64_t V, void* scratch,
+                                    size_t scratch_bytes, void* stream);
+size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t V);
+
 /* AdamW update of one parameter tensor in place, moments m and v in device
  * memory, step count t >= 1. Replaces Tensor::adamw_step (tensor.rs:931-1023,
  * whose device path copies the parameter to the host and back) with the same

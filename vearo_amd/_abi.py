@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import numpy as np
 
@@ -78,6 +78,7 @@ class DevicePanic(VhError):
 
 
 fp = c_void_p  # device pointers travel as void*
+LP = POINTER(VhLayout)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -172,6 +173,38 @@ SIGNATURES = {
          POINTER(VhLayout), fp, POINTER(VhLayout), fp, POINTER(VhLayout), fp, POINTER(VhLayout),
          c_void_p, c_size_t, c_void_p],
     ),
+    "vh_qk_norm_rope_fwd": (c_int, [fp, LP, fp, LP, fp, fp, fp, c_float, c_double, c_int32, c_int32, fp, LP, fp, LP, c_void_p]),
+    "vh_qk_norm_rope_bwd": (
+        c_int,
+        [fp, LP, fp, LP, fp, fp, fp, c_float, c_double, c_int32, c_int32, fp, LP, fp, LP, fp, LP, fp, LP, fp, fp,
+         c_void_p, c_size_t, c_void_p],
+    ),
+    "vh_qk_norm_rope_bwd_scratch_bytes": (c_size_t, [c_int64, c_int64]),
+    "vh_packed_attention_fwd": (
+        c_int,
+        [fp, LP, fp, LP, fp, LP, fp, c_int64, c_float, c_int, fp, LP, fp, c_void_p, c_size_t, c_void_p],
+    ),
+    "vh_packed_attention_bwd": (
+        c_int,
+        [fp, LP, fp, LP, fp, LP, fp, c_int64, c_float, c_int, fp, LP, fp, fp, LP, fp, LP, fp, LP, fp, LP, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "vh_packed_attention_scratch_bytes": (c_size_t, [c_int64] * 5 + [c_int]),
+    "vh_linear_cross_entropy_fwd": (
+        c_int,
+        [fp, c_int64, fp, c_int64, fp, c_float, fp, fp, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p],
+    ),
+    "vh_linear_cross_entropy_bwd": (
+        c_int,
+        [fp, c_int64, fp, c_int64, fp, c_float, fp, fp, fp, c_int64, fp, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "vh_linear_cross_entropy_fwd_bwd": (
+        c_int,
+        [fp, c_int64, fp, c_int64, fp, c_float, fp, fp, fp, c_int64, fp, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "vh_linear_cross_entropy_scratch_bytes": (c_size_t, [c_int64, c_int64]),
     "vh_adamw_step": (
         c_int,
         [fp, fp, fp, fp, c_int64, c_int32, c_float, c_float, c_float, c_float, c_float, c_void_p],

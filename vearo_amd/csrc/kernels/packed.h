@@ -1,0 +1,250 @@
+// packed.h -- attention over packed sequences with grouped heads, forward and
+// backward: the tables, and the row kernels that take any head size and any values.
+//
+// T tokens hold n sequences one behind the other, sequence s the tokens
+// starts[s] .. starts[s + 1] - 1; query head h reads key head h / (Hq / Hk). Within a
+// sequence, with j <= i where causal:
+//   s_ij = scale q_i k_j,  P_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij),
+//   o_i = sum_j P_ij v_j
+//   D_i = do_i o_i,  dS_ij = P_ij (do_i v_j - D_i),
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij do_i,
+// the sums over i also over the query heads of the key head. Masked pairs are not
+// formed at all, so what an unseen token holds (infinities, NaN) reaches no other row.
+#pragma once
+#include "common.h"
+
+// Running totals of tiles (64 rows) and blocks (a.block_rows) over the sequences, 256
+// sequences a step: ends with *found = tile `idx` and *block = block `idx` where there
+// are so many, and in ALL form with the totals in `tot` and every bad start reported.
+// A start that is negative, before its predecessor or past T gives its sequence no rows.
+struct PaFind {
+  int wave[4][2];
+  int bad;
+  PaSpan tile, block;
+};
+template <bool ALL>
+VH_DEV void pa_find(const PaArgs& a, int idx, PaFind& f, int (&tot)[2]) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  tot[0] = tot[1] = 0;
+  if (tid == 0) {
+    f.bad = 0;
+    f.tile.len = f.block.len = -1;
+  }
+  __syncthreads();
+  for (int base = 0; base < a.n; base += 256) {
+    const int i = base + tid;
+    int start = 0, len = 0;
+    if (i < a.n) {
+      const int s0 = a.starts[i], s1 = a.starts[i + 1];
+      const bool first = i > 0 || (s0 >= 0 && s0 <= a.T), ok = s0 >= 0 && s1 >= s0 && s1 <= a.T;
+      if (ok) {
+        start = s0;
+        len = s1 - s0;
+      } else if (ALL) {
+        f.bad = 1;
+        const int at = first ? i + 1 : 0, v = first ? s1 : s0;
+        atomicMin(&a.err->start, ((unsigned long long)(uint32_t)at << 32) | (uint32_t)v);
+        a.err->start_bound = (unsigned)a.T;
+      }
+    }
+    const int c0 = (len + 63) >> 6, c1 = (len + a.block_rows - 1) / a.block_rows;
+    int x0 = c0, x1 = c1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y0 = __shfl_up(x0, o, 64), y1 = __shfl_up(x1, o, 64);
+      if (lane >= o) {
+        x0 += y0;
+        x1 += y1;
+      }
+    }
+    if (lane == 63) {
+      f.wave[w][0] = x0;
+      f.wave[w][1] = x1;
+    }
+    __syncthreads();
+    int e0 = tot[0] + x0 - c0, e1 = tot[1] + x1 - c1;
+    for (int k = 0; k < w; ++k) {
+      e0 += f.wave[k][0];
+      e1 += f.wave[k][1];
+    }
+    if (idx >= e0 && idx < e0 + c0) f.tile = PaSpan{start, len, (idx - e0) * 64, e0};
+    if (idx >= e1 && idx < e1 + c1) f.block = PaSpan{start, len, (idx - e1) * a.block_rows, e0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      tot[0] += f.wave[k][0];
+      tot[1] += f.wave[k][1];
+    }
+    __syncthreads();
+    if (!ALL && tot[0] > idx && tot[1] > idx) break;
+  }
+}
+
+// Writes entry blockIdx.x of the tables; workgroup 0 also the header. A bad start
+// leaves the header without tiles: the launches that follow then do nothing.
+VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
+  int tot[2];
+  if (idx == 0) {
+    pa_find<true>(a, idx, f, tot);
+    if (threadIdx.x == 0) {
+      a.head->ntiles = f.bad ? 0 : tot[0];
+      a.head->nblocks = f.bad ? 0 : tot[1];
+    }
+  } else {
+    pa_find<false>(a, idx, f, tot);
+  }
+  if (threadIdx.x == 0) {
+    if (f.tile.len >= 0 && idx < a.max_tiles) a.tiles[idx] = f.tile;
+    if (f.block.len >= 0 && idx < a.max_blocks) a.blocks[idx] = f.block;
+  }
+}
+
+VH_DEV void pa_plan_impl(const PaArgs& a) {
+  __shared__ PaFind f;
+  pa_tables(a, blockIdx.x, f);
+}
+
+// ------------------------------------------------------------ row kernels --
+// A wave per row, keys over its lanes for the scores, elements over its lanes for
+// the products. Scores are formed again in each pass instead of kept, so a row may
+// have any length. f32 arithmetic throughout, element by element, nothing masked
+// ever touched. These carry head sizes past 128 and, inside the matrix kernels,
+// blocks whose values those cannot hold; a row costs its dot products (about a
+// tenth of the vector units' rate, each lane reading its own key's row).
+
+// An LDS row of up to 256 elements that the wave alone reads and writes.
+VH_DEV void pa_row_to_lds(float* l, const float* p, int D) {
+  const int lane = threadIdx.x & 63;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int d = lane; d < D; d += 64) l[d] = p[d];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+VH_DEV float pa_dot(const float* l, const float* p, int D) {
+  float s = 0.0f;
+  for (int d = 0; d < D; ++d) s = fmaf(l[d], p[d], s);
+  return s;
+}
+VH_DEV float pa_lane(float v, int j) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
+}
+// acc[u] += sum over the wave's m live lanes j of c_j x[row j][lane + 64 u].
+VH_DEV void pa_axpy(float c, const float* x, int64_t st, int m, int D, float (&acc)[4]) {
+  const int lane = threadIdx.x & 63;
+  for (int j = 0; j < m; ++j) {
+    const float cj = pa_lane(c, j);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (lane + 64 * u < D) acc[u] = fmaf(cj, x[j * st + lane + 64 * u], acc[u]);
+  }
+}
+
+VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, float* l) {
+  const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
+  const int64_t tok = (int64_t)sp.start + i;
+  const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
+  const float* v = a.v.p + sp.start * a.v.st + hk * a.v.sh;
+  const int nk = a.causal ? i + 1 : sp.len;
+  pa_row_to_lds(l, a.q.p + tok * a.q.st + h * a.q.sh, a.D);
+  float m = -INFINITY;
+  for (int j = lane; j < nk; j += 64) m = fmaxf(m, pa_dot(l, k + j * a.k.st, a.D) * a.scale);
+  m = group_max<64>(m);
+  float sum = 0.0f, acc[4] = {};
+  for (int j0 = 0; j0 < nk; j0 += 64) {
+    float p = 0.0f;
+    if (j0 + lane < nk) p = expf(pa_dot(l, k + (j0 + lane) * a.k.st, a.D) * a.scale - m);
+    sum += p;
+    pa_axpy(p, v + j0 * a.v.st, a.v.st, min(64, nk - j0), a.D, acc);
+  }
+  sum = group_sum<64>(sum);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + 64 * u < a.D) a.out[tok * a.out_t + h * a.out_h + lane + 64 * u] = acc[u] / sum;
+  if (lane == 0) a.lse[(int64_t)h * a.T + tok] = m + logf(sum);
+}
+
+VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, float* l, float* lg) {
+  const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
+  const int64_t tok = (int64_t)sp.start + i;
+  const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
+  const float* v = a.v.p + sp.start * a.v.st + hk * a.v.sh;
+  const int nk = a.causal ? i + 1 : sp.len;
+  pa_row_to_lds(l, a.q.p + tok * a.q.st + h * a.q.sh, a.D);
+  pa_row_to_lds(lg, a.g.p + tok * a.g.st + h * a.g.sh, a.D);
+  const float lse = a.lse[(int64_t)h * a.T + tok], dl = a.delta[(int64_t)h * a.T + tok];
+  float acc[4] = {};
+  for (int j0 = 0; j0 < nk; j0 += 64) {
+    float ds = 0.0f;
+    if (const int64_t j = j0 + lane; j < nk) {
+      const float p = expf(pa_dot(l, k + j * a.k.st, a.D) * a.scale - lse);
+      ds = p * (pa_dot(lg, v + j * a.v.st, a.D) - dl);
+    }
+    pa_axpy(ds, k + j0 * a.k.st, a.k.st, min(64, nk - j0), a.D, acc);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + 64 * u < a.D) a.dq[tok * a.dq_t + h * a.dq_h + lane + 64 * u] = acc[u] * a.scale;
+}
+
+VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float* l, float* lv) {
+  const int lane = threadIdx.x & 63, G = a.q.H / a.k.H;
+  const int64_t tok = (int64_t)sp.start + j;
+  pa_row_to_lds(l, a.k.p + tok * a.k.st + hk * a.k.sh, a.D);
+  pa_row_to_lds(lv, a.v.p + tok * a.v.st + hk * a.v.sh, a.D);
+  float dk[4] = {}, dv[4] = {};
+  for (int h = hk * G; h < (hk + 1) * G; ++h) {
+    const float* q = a.q.p + sp.start * a.q.st + h * a.q.sh;
+    const float* g = a.g.p + sp.start * a.g.st + h * a.g.sh;
+    const int64_t at = (int64_t)h * a.T + sp.start;
+    for (int i0 = a.causal ? j : 0; i0 < sp.len; i0 += 64) {
+      float p = 0.0f, ds = 0.0f;
+      if (const int64_t i = i0 + lane; i < sp.len) {
+        p = expf(pa_dot(l, q + i * a.q.st, a.D) * a.scale - a.lse[at + i]);
+        ds = p * (pa_dot(lv, g + i * a.g.st, a.D) - a.delta[at + i]);
+      }
+      const int m = min(64, sp.len - i0);
+      pa_axpy(ds, q + i0 * a.q.st, a.q.st, m, a.D, dk);
+      pa_axpy(p, g + i0 * a.g.st, a.g.st, m, a.D, dv);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + 64 * u < a.D) {
+      a.dk[tok * a.dk_t + hk * a.dk_h + lane + 64 * u] = dk[u] * a.scale;
+      a.dv[tok * a.dv_t + hk * a.dv_h + lane + 64 * u] = dv[u];
+    }
+}
+
+// The rows of one block, over the workgroup's waves. MODE 0 forward, 1 dq, 2 dk and dv.
+template <int MODE>
+VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, float (*l)[2][VH_PA_MAX_D]) {
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int end = min(sp.len, sp.row0 + a.block_rows);
+  for (int i = sp.row0 + w; i < end; i += nw) {
+    if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l[w][0]);
+    if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l[w][0], l[w][1]);
+    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l[w][0], l[w][1]);
+  }
+}
+// Grid: (blocks, heads: of q, or of k for dk and dv).
+template <int MODE>
+VH_DEV void pa_rows_impl(const PaArgs& a) {
+  __shared__ float l[4][2][VH_PA_MAX_D];
+  if ((int)blockIdx.x >= a.head->nblocks) return;
+  pa_rows<MODE>(a, blockIdx.y, a.blocks[blockIdx.x], l);
+}
+
+// delta[h][t] = sum over d of dout * out for every row of the sequences, a wave per row
+// of 64-row tile blockIdx.x and head blockIdx.y.
+VH_DEV void pa_delta_impl(const PaArgs& a) {
+  if ((int)blockIdx.x >= a.head->ntiles) return;
+  const PaSpan sp = a.tiles[blockIdx.x];
+  const int lane = threadIdx.x & 63, h = blockIdx.y;
+  for (int i = sp.row0 + (threadIdx.x >> 6); i < min(sp.len, sp.row0 + 64); i += 4) {
+    const int64_t tok = (int64_t)sp.start + i;
+    const float* o = a.o.p + tok * a.o.st + h * a.o.sh;
+    const float* g = a.g.p + tok * a.g.st + h * a.g.sh;
+    float s = 0.0f;
+    for (int d = lane; d < a.D; d += 64) s = fmaf(o[d], g[d], s);
+    s = group_sum<64>(s);
+    if (lane == 0) a.delta[(int64_t)h * a.T + tok] = s;
+  }
+}

@@ -1,0 +1,26 @@
+// packed_kernels.hip -- the second code object that libvearo_hip.so embeds: the
+// operators of packed training (query / key norm and rotation, attention over packed
+// sequences, cross-entropy of a linear layer). Same conventions as vearo_kernels.hip.
+#include "linxent.h"
+#include "packed.h"
+#include "rope.h"
+
+// Query / key norm and rotation: vh_rope_{fwd,bwd}_v<VW>_l<lanes per row>_n<slots per lane>
+#define K_ROPE(VW, L, N)                                                                                            \
+  extern "C" __global__ void __launch_bounds__(256) vh_rope_fwd_v##VW##_l##L##_n##N(RopeArgs a) { rope_fwd_impl<VW, L, N>(a); } \
+  extern "C" __global__ void __launch_bounds__(256) vh_rope_bwd_v##VW##_l##L##_n##N(RopeArgs a) { rope_bwd_impl<VW, L, N>(a); }
+K_ROPE(4, 4, 1) K_ROPE(4, 8, 1) K_ROPE(4, 16, 1) K_ROPE(4, 32, 1) K_ROPE(1, 64, 1) K_ROPE(1, 64, 2)
+
+// Attention over packed sequences: tables, row kernels.
+extern "C" __global__ void __launch_bounds__(256) vh_pa_plan(PaArgs a) { pa_plan_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_pa_delta(PaArgs a) { pa_delta_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_fwd(PaArgs a) { pa_rows_impl<0>(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_dq(PaArgs a) { pa_rows_impl<1>(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_dkdv(PaArgs a) { pa_rows_impl<2>(a); }
+
+// Cross-entropy of a linear layer.
+extern "C" __global__ void __launch_bounds__(1024) vh_lx_count(LxCountArgs a) { lx_count_impl(a); }
+extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_stats(LxArgs a) { lx_row_impl<true, false>(a); }
+extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_grad(LxArgs a) { lx_row_impl<false, true>(a); }
+extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_stats_grad(LxArgs a) { lx_row_impl<true, true>(a); }
+extern "C" __global__ void __launch_bounds__(1024) vh_lx_loss(LxLossArgs a) { lx_loss_impl(a); }

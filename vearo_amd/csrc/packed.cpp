@@ -1,0 +1,448 @@
+// packed.cpp -- host side of the packed-training operators (include/vearo_hip.h): the
+// norm and rotation of queries and keys, attention over packed sequences, and the
+// cross-entropy of a linear layer. Arguments are checked here, and every size and
+// alignment a kernel assumes, before anything is launched.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "rt_internal.h"
+#include "vh_kargs.h"
+
+using vh_rt::CallScratch;
+using vh_rt::fail;
+
+#define VH_TRY(expr)              \
+  do {                            \
+    int rc_ = (expr);             \
+    if (rc_ != VH_OK) return rc_; \
+  } while (0)
+
+namespace {
+
+template <typename A>
+int launch(const std::string& name, int64_t gx, int64_t gy, int64_t gz, unsigned block, hipStream_t s, A args) {
+  return vh_rt::launch_args(name, gx, gy, gz, block, s, &args);
+}
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Heads {
+  int64_t T = 0, H = 0, D = 0;
+};
+
+// A [T, H, D] layout with unit stride on D; `like` (if given) fixes T, D and, with
+// same_heads, H. Outputs must not map two elements to one address by a zero stride.
+int heads_of(const vh_layout* l, const std::string& what, bool output, const Heads* like, bool same_heads, Heads* out) {
+  VH_TRY(vh_rt::check_layout(l, what.c_str()));
+  if (l->rank != 3) return fail(VH_ERR_INVALID, what + ": expected a rank-3 [T, H, D] layout");
+  const Heads h{l->dims[0], l->dims[1], l->dims[2]};
+  if (like && (h.T != like->T || h.D != like->D || (same_heads && h.H != like->H)))
+    return fail(VH_ERR_INVALID, what + ": shape does not match");
+  if (l->strides[2] != 1 && h.D > 1) return fail(VH_ERR_UNSUPPORTED, what + ": the last dim must have unit stride");
+  if (output && h.T * h.H > 0 && ((l->strides[0] == 0 && h.T > 1) || (l->strides[1] == 0 && h.H > 1)))
+    return fail(VH_ERR_INVALID, what + ": an output cannot be broadcast");
+  if (out) *out = h;
+  return VH_OK;
+}
+
+// Rows may be read and written as 16-byte units.
+bool rows16(const void* p, const vh_layout* l) {
+  return aligned16(p) && l->dims[2] % 4 == 0 && (l->strides[0] % 4 == 0 || l->dims[0] <= 1) &&
+         (l->strides[1] % 4 == 0 || l->dims[1] <= 1);
+}
+
+// -------------------------------------------------------- query / key rotation --
+struct RopeCfg {
+  int vw, lpr, ns;
+  std::string suffix() const {
+    return "_v" + std::to_string(vw) + "_l" + std::to_string(lpr) + "_n" + std::to_string(ns);
+  }
+};
+// 16-byte units where every row allows them and pairs do not straddle one; a team's lanes
+// hold eight elements each. Else one pair per lane and slot.
+RopeCfg rope_cfg(int64_t D, int64_t R, bool vec) {
+  if (vec && R % 8 == 0) return {4, D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, 1};
+  return {1, 64, D <= 128 ? 1 : 2};
+}
+constexpr int64_t kRopeBwdBlocks = 1024;
+
+int rope_args(const char* fn, const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
+              const float* wk, const float* positions, float eps, double base, int32_t rotary, int32_t interleaved,
+              RopeArgs* a, Heads* hq, Heads* hk, bool* vec) {
+  const std::string f = fn;
+  VH_TRY(heads_of(ql, f + " q", false, nullptr, false, hq));
+  VH_TRY(heads_of(kl, f + " k", false, hq, false, hk));
+  if (hq->D < 1 || hq->D > VH_ROPE_MAX_D)
+    return fail(VH_ERR_UNSUPPORTED, f + ": head size must be in [1, " + std::to_string(VH_ROPE_MAX_D) + "]");
+  if (rotary < 0 || rotary > hq->D || rotary % 2)
+    return fail(VH_ERR_INVALID, f + ": rotary must be even and in [0, D]");
+  if (!(eps >= 0.0f)) return fail(VH_ERR_INVALID, f + ": eps must not be negative");
+  if (!(base > 0.0) || !std::isfinite(base)) return fail(VH_ERR_INVALID, f + ": base must be positive and finite");
+  if (hq->H > INT32_MAX / 2 || hk->H > INT32_MAX / 2) return fail(VH_ERR_UNSUPPORTED, f + ": head count exceeds int32");
+  if (hq->T > 0 && (!wq || !wk || !positions || (hq->H && !q) || (hk->H && !k)))
+    return fail(VH_ERR_INVALID, f + ": null pointer");
+  *a = RopeArgs{};
+  a->x[0] = q;
+  a->x[1] = k;
+  a->w[0] = wq;
+  a->w[1] = wk;
+  a->xt[0] = ql->strides[0];
+  a->xt[1] = kl->strides[0];
+  a->xh[0] = ql->strides[1];
+  a->xh[1] = kl->strides[1];
+  a->H[0] = (int32_t)hq->H;
+  a->H[1] = (int32_t)hk->H;
+  a->positions = positions;
+  a->T = hq->T;
+  a->D = (int32_t)hq->D;
+  a->R = rotary;
+  a->interleaved = interleaved != 0;
+  a->eps = eps;
+  for (int i = 0; i < rotary / 2; ++i) a->rate[i] = std::pow(base, -2.0 * i / rotary) / 3.14159265358979323846;
+  *vec = rows16(q, ql) && rows16(k, kl) && aligned16(wq) && aligned16(wk);
+  return VH_OK;
+}
+
+void rope_out(RopeArgs* a, float* yq, const vh_layout* qol, float* yk, const vh_layout* kol) {
+  a->y[0] = yq;
+  a->y[1] = yk;
+  a->yt[0] = qol->strides[0];
+  a->yt[1] = kol->strides[0];
+  a->yh[0] = qol->strides[1];
+  a->yh[1] = kol->strides[1];
+}
+
+// ------------------------------------------------------------ packed attention --
+int64_t pa_units(int64_t T, int64_t n, int64_t rows) { return T / rows + n; }
+
+// The workspace, in the order its parts are laid out.
+struct PaScratch {
+  size_t head, tiles, blocks, delta, total;
+  PaScratch(int64_t T, int64_t n, int64_t Hq, int64_t block_rows, bool backward) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t p = at;
+      at += align256(bytes);
+      return p;
+    };
+    head = take(sizeof(PaHead));
+    tiles = take(sizeof(PaSpan) * (size_t)pa_units(T, n, 64));
+    blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, n, block_rows));
+    delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
+    total = at;
+  }
+};
+constexpr int kPaBlockRows = 64;
+
+PaTensor pa_tensor(const float* p, const vh_layout* l) {
+  return PaTensor{p, l->strides[0], l->strides[1], (int32_t)l->dims[1], rows16(p, l) ? 1 : 0};
+}
+
+struct PaCall {
+  PaArgs a{};
+  Heads q, k;
+  bool empty = false;
+};
+
+int pa_check(const std::string& f, const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
+             const vh_layout* vl, const int32_t* starts, int64_t n, float scale, int causal, const float* out,
+             const vh_layout* ol, const float* lse, PaCall* c) {
+  VH_TRY(heads_of(ql, f + " q", false, nullptr, false, &c->q));
+  VH_TRY(heads_of(kl, f + " k", false, &c->q, false, &c->k));
+  VH_TRY(heads_of(vl, f + " v", false, &c->k, true, nullptr));
+  VH_TRY(heads_of(ol, f + " out", true, &c->q, true, nullptr));
+  const int64_t T = c->q.T, D = c->q.D;
+  if (n < 0) return fail(VH_ERR_INVALID, f + ": negative sequence count");
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(VH_ERR_INVALID, f + ": scale must be positive and finite");
+  if (D < 1 || D > VH_PA_MAX_D)
+    return fail(VH_ERR_UNSUPPORTED, f + ": head size must be in [1, " + std::to_string(VH_PA_MAX_D) + "]");
+  if (c->k.H == 0 ? c->q.H != 0 : c->q.H % c->k.H != 0)
+    return fail(VH_ERR_INVALID, f + ": query heads must be a multiple of key heads");
+  if (T > INT32_MAX - 256 || n > INT32_MAX / 2 || c->q.H > 65535)
+    return fail(VH_ERR_UNSUPPORTED, f + ": size outside the implemented range");
+  c->empty = T == 0 || n == 0 || c->q.H == 0;
+  if (c->empty) return VH_OK;
+  if (!q || !k || !v || !starts || !out || !lse) return fail(VH_ERR_INVALID, f + ": null pointer");
+  PaArgs& a = c->a;
+  a.q = pa_tensor(q, ql);
+  a.k = pa_tensor(k, kl);
+  a.v = pa_tensor(v, vl);
+  a.starts = starts;
+  a.err = vh_rt::error_record();
+  a.n = (int32_t)n;
+  a.T = (int32_t)T;
+  a.D = (int32_t)D;
+  a.block_rows = kPaBlockRows;
+  a.max_tiles = (int32_t)std::min<int64_t>(pa_units(T, n, 64), INT32_MAX);
+  a.max_blocks = (int32_t)std::min<int64_t>(pa_units(T, n, a.block_rows), INT32_MAX);
+  a.causal = causal != 0;
+  a.scale = scale;
+  return VH_OK;
+}
+
+void pa_place(PaArgs* a, const PaScratch& l, void* base) {
+  char* p = static_cast<char*>(base);
+  a->head = reinterpret_cast<PaHead*>(p + l.head);
+  a->tiles = reinterpret_cast<PaSpan*>(p + l.tiles);
+  a->blocks = reinterpret_cast<PaSpan*>(p + l.blocks);
+  a->delta = reinterpret_cast<float*>(p + l.delta);
+}
+
+// ------------------------------------------------- cross-entropy of a linear layer --
+constexpr size_t kLxPieceBytes = size_t(256) << 20;
+int64_t lx_ld(int64_t V) { return (V + 3) / 4 * 4; }
+// Rows per piece: whole 256-row product tiles within kLxPieceBytes, one at least.
+int64_t lx_rows(int64_t R, int64_t V) {
+  const int64_t fit = (int64_t)(kLxPieceBytes / (sizeof(float) * (size_t)lx_ld(V))) / 256 * 256;
+  return std::min<int64_t>(R, std::max<int64_t>(fit, 256));
+}
+struct LxScratch {
+  size_t z, row_loss, inv, total;
+  LxScratch(int64_t R, int64_t V) {
+    z = 0;
+    row_loss = align256(sizeof(float) * (size_t)(lx_rows(R, V) * lx_ld(V)));
+    inv = row_loss + align256(sizeof(float) * (size_t)R);
+    total = inv + 256;
+  }
+};
+
+struct LxCall {
+  const float *x, *w, *targets, *grad_out;
+  int64_t ldx, ldw, lddx, lddw, R, D, V;
+  float ignore;
+  float *loss, *stats, *dx, *dw;
+  bool forward, backward;
+};
+
+int lx_product(int64_t M, int64_t N, int64_t K, const float* a, int64_t a_sm, int64_t a_sk, const float* b, int64_t b_sk,
+               int64_t b_sn, float* c, int64_t ldc, bool accumulate, hipStream_t s) {
+  vh_gemm_desc d{};
+  d.M = M;
+  d.N = N;
+  d.K = K;
+  d.a = a;
+  d.a_sm = a_sm;
+  d.a_sk = a_sk;
+  d.b = b;
+  d.b_sk = b_sk;
+  d.b_sn = b_sn;
+  d.c = c;
+  d.c_sm = ldc;
+  d.batch[0] = d.batch[1] = 1;
+  d.alpha = 1.0f;
+  d.accumulate = accumulate;
+  return vh_gemm(&d, s);
+}
+
+int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes, void* stream) {
+  const std::string f = fn;
+  if (c.R <= 0) return fail(VH_ERR_INVALID, f + ": rows must be > 0");
+  if (c.V <= 0) return fail(VH_ERR_INVALID, f + ": vocabulary must be > 0");
+  if (c.D <= 0) return fail(VH_ERR_INVALID, f + ": width must be > 0");
+  if (c.ldx < c.D || c.ldw < c.D || (c.backward && (c.lddx < c.D || c.lddw < c.D)))
+    return fail(VH_ERR_INVALID, f + ": row stride below D");
+  if (!c.x || !c.w || !c.targets || (c.forward && !c.loss) || (c.backward && (!c.grad_out || !c.dx || !c.dw)) ||
+      (!(c.forward && c.backward) && !c.stats))
+    return fail(VH_ERR_INVALID, f + ": null pointer");
+  if (reinterpret_cast<uintptr_t>(c.stats) % 8 != 0)
+    return fail(VH_ERR_INVALID, f + ": row_stats must be 8-byte aligned");
+  if (c.R > INT32_MAX || c.V > INT32_MAX - 4 || c.D > INT32_MAX)
+    return fail(VH_ERR_UNSUPPORTED, f + ": size exceeds int32");
+  VH_TRY(vh_rt::require_init());
+  hipStream_t s = vh_rt::stream_of(stream);
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
+    return fail(VH_ERR_UNSUPPORTED, f + ": cannot run under graph capture");
+  const LxScratch lay(c.R, c.V);
+  CallScratch sc;
+  VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
+  char* base = static_cast<char*>(sc.p);
+  float* z = reinterpret_cast<float*>(base + lay.z);
+  float* row_loss = reinterpret_cast<float*>(base + lay.row_loss);
+  float* inv = reinterpret_cast<float*>(base + lay.inv);
+  const int64_t ld = lx_ld(c.V), piece = lx_rows(c.R, c.V);
+  VH_TRY(launch("vh_lx_count", 1, 1, 1, 1024, s,
+                LxCountArgs{c.targets, inv, vh_rt::error_record(), c.R, (int32_t)c.V, c.ignore}));
+  const char* kernel = c.forward ? (c.backward ? "vh_lx_stats_grad" : "vh_lx_stats") : "vh_lx_grad";
+  for (int64_t r = 0; r < c.R; r += piece) {
+    const int64_t rows = std::min(piece, c.R - r);
+    const float* x = c.x + r * c.ldx;
+    VH_TRY(lx_product(rows, c.V, c.D, x, c.ldx, 1, c.w, 1, c.ldw, z, ld, false, s));
+    VH_TRY(launch(kernel, rows, 1, 1, 512, s,
+                  LxArgs{z, c.targets + r, c.grad_out, inv, c.stats ? c.stats + 2 * r : nullptr,
+                         c.forward ? row_loss + r : nullptr, rows, ld, (int32_t)c.V, c.ignore}));
+    if (!c.backward) continue;
+    VH_TRY(lx_product(rows, c.D, c.V, z, ld, 1, c.w, c.ldw, 1, c.dx + r * c.lddx, c.lddx, false, s));
+    VH_TRY(lx_product(c.V, c.D, rows, z, 1, ld, x, c.ldx, 1, c.dw, c.lddw, r > 0, s));
+  }
+  if (c.forward) VH_TRY(launch("vh_lx_loss", 1, 1, 1, 1024, s, LxLossArgs{row_loss, inv, c.loss, c.R}));
+  return VH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vh_qk_norm_rope_fwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
+                        const float* wk, const float* positions, float eps, double base, int32_t rotary,
+                        int32_t interleaved, float* qo, const vh_layout* qol, float* ko, const vh_layout* kol,
+                        void* stream) {
+  RopeArgs a;
+  Heads hq, hk;
+  bool vec;
+  VH_TRY(rope_args("vh_qk_norm_rope_fwd", q, ql, k, kl, wq, wk, positions, eps, base, rotary, interleaved, &a, &hq, &hk,
+                   &vec));
+  VH_TRY(heads_of(qol, "vh_qk_norm_rope_fwd qo", true, &hq, true, nullptr));
+  VH_TRY(heads_of(kol, "vh_qk_norm_rope_fwd ko", true, &hk, true, nullptr));
+  const int64_t H = hq.H + hk.H;
+  if (hq.T == 0 || H == 0) return vh_rt::require_init();
+  if ((hq.H && !qo) || (hk.H && !ko)) return fail(VH_ERR_INVALID, "vh_qk_norm_rope_fwd: null pointer");
+  VH_TRY(vh_rt::require_init());
+  rope_out(&a, qo, qol, ko, kol);
+  const RopeCfg c = rope_cfg(hq.D, rotary, vec && rows16(qo, qol) && rows16(ko, kol));
+  a.heads_per = hq.T * c.lpr * cdiv(H, 8) < (int64_t(1) << 19) ? 4 : 8;
+  return launch("vh_rope_fwd" + c.suffix(), cdiv(hq.T, 256 / c.lpr), cdiv(H, a.heads_per), 1, 256,
+                vh_rt::stream_of(stream), a);
+}
+
+size_t vh_qk_norm_rope_bwd_scratch_bytes(int64_t T, int64_t D) {
+  if (T <= 0 || D <= 0) return 0;
+  return align256(sizeof(float) * 2 * (size_t)(D * std::min<int64_t>(cdiv(T, 4), kRopeBwdBlocks)));
+}
+
+int vh_qk_norm_rope_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
+                        const float* wk, const float* positions, float eps, double base, int32_t rotary,
+                        int32_t interleaved, const float* dqo, const vh_layout* dqol, const float* dko,
+                        const vh_layout* dkol, float* dq, const vh_layout* dql, float* dk, const vh_layout* dkl,
+                        float* dwq, float* dwk, void* scratch, size_t scratch_bytes, void* stream) {
+  RopeArgs a;
+  Heads hq, hk;
+  bool vec;
+  VH_TRY(rope_args("vh_qk_norm_rope_bwd", q, ql, k, kl, wq, wk, positions, eps, base, rotary, interleaved, &a, &hq, &hk,
+                   &vec));
+  VH_TRY(heads_of(dqol, "vh_qk_norm_rope_bwd dqo", false, &hq, true, nullptr));
+  VH_TRY(heads_of(dkol, "vh_qk_norm_rope_bwd dko", false, &hk, true, nullptr));
+  VH_TRY(heads_of(dql, "vh_qk_norm_rope_bwd dq", true, &hq, true, nullptr));
+  VH_TRY(heads_of(dkl, "vh_qk_norm_rope_bwd dk", true, &hk, true, nullptr));
+  if (!dwq || !dwk || (hq.T && ((hq.H && (!dqo || !dq)) || (hk.H && (!dko || !dk)))))
+    return fail(VH_ERR_INVALID, "vh_qk_norm_rope_bwd: null pointer");
+  VH_TRY(vh_rt::require_init());
+  hipStream_t s = vh_rt::stream_of(stream);
+  if (hq.T == 0 || hq.H + hk.H == 0) {  // sums over nothing
+    VH_TRY(vh_fill_f32(dwq, 0.0f, hq.D, s));
+    return vh_fill_f32(dwk, 0.0f, hq.D, s);
+  }
+  rope_out(&a, dq, dql, dk, dkl);
+  a.dy[0] = dqo;
+  a.dy[1] = dko;
+  a.dt[0] = dqol->strides[0];
+  a.dt[1] = dkol->strides[0];
+  a.dh[0] = dqol->strides[1];
+  a.dh[1] = dkol->strides[1];
+  const RopeCfg c = rope_cfg(hq.D, rotary, vec && rows16(dqo, dqol) && rows16(dko, dkol) && rows16(dq, dql) && rows16(dk, dkl));
+  const int64_t blocks = std::min<int64_t>(cdiv(hq.T, 256 / c.lpr), kRopeBwdBlocks);
+  CallScratch sc;
+  VH_TRY(sc.get(s, scratch, scratch_bytes, vh_qk_norm_rope_bwd_scratch_bytes(hq.T, hq.D)));
+  a.part = static_cast<float*>(sc.p);
+  VH_TRY(launch("vh_rope_bwd" + c.suffix(), blocks, 1, 1, 256, s, a));
+  ColReduceArgs r{a.part, dwq, dwk, (int32_t)blocks, a.D, 2};
+  return launch("vh_col_reduce", cdiv(hq.D, VH_COLR_COLS), 2, 1, VH_COLR_COLS * 16, s, r);
+}
+
+size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D, int backward) {
+  if (T <= 0 || n <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return 0;
+  return PaScratch(T, n, Hq, kPaBlockRows, backward != 0).total;
+}
+
+int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
+                            const vh_layout* vl, const int32_t* starts, int64_t n, float scale, int causal, float* out,
+                            const vh_layout* ol, float* lse, void* scratch, size_t scratch_bytes, void* stream) {
+  PaCall c;
+  VH_TRY(pa_check("vh_packed_attention_fwd", q, ql, k, kl, v, vl, starts, n, scale, causal, out, ol, lse, &c));
+  VH_TRY(vh_rt::require_init());
+  if (c.empty) return VH_OK;
+  PaArgs& a = c.a;
+  a.out = out;
+  a.out_t = ol->strides[0];
+  a.out_h = ol->strides[1];
+  a.lse = lse;
+  hipStream_t s = vh_rt::stream_of(stream);
+  const PaScratch lay(c.q.T, n, c.q.H, a.block_rows, false);
+  CallScratch sc;
+  VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
+  pa_place(&a, lay, sc.p);
+  VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
+  return launch("vh_pa_rows_fwd", a.max_blocks, c.q.H, 1, 256, s, a);
+}
+
+int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
+                            const vh_layout* vl, const int32_t* starts, int64_t n, float scale, int causal,
+                            const float* out, const vh_layout* ol, const float* lse, const float* dout,
+                            const vh_layout* dol, float* dq, const vh_layout* dql, float* dk, const vh_layout* dkl,
+                            float* dv, const vh_layout* dvl, void* scratch, size_t scratch_bytes, void* stream) {
+  const std::string f = "vh_packed_attention_bwd";
+  PaCall c;
+  VH_TRY(pa_check(f, q, ql, k, kl, v, vl, starts, n, scale, causal, out, ol, lse, &c));
+  VH_TRY(heads_of(dol, f + " dout", false, &c.q, true, nullptr));
+  VH_TRY(heads_of(dql, f + " dq", true, &c.q, true, nullptr));
+  VH_TRY(heads_of(dkl, f + " dk", true, &c.k, true, nullptr));
+  VH_TRY(heads_of(dvl, f + " dv", true, &c.k, true, nullptr));
+  if (!c.empty && (!dout || !dq || !dk || !dv)) return fail(VH_ERR_INVALID, f + ": null pointer");
+  VH_TRY(vh_rt::require_init());
+  if (c.empty) return VH_OK;
+  PaArgs& a = c.a;
+  a.o = pa_tensor(out, ol);
+  a.g = pa_tensor(dout, dol);
+  a.lse = const_cast<float*>(lse);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.dq_t = dql->strides[0];
+  a.dq_h = dql->strides[1];
+  a.dk_t = dkl->strides[0];
+  a.dk_h = dkl->strides[1];
+  a.dv_t = dvl->strides[0];
+  a.dv_h = dvl->strides[1];
+  hipStream_t s = vh_rt::stream_of(stream);
+  const PaScratch lay(c.q.T, n, c.q.H, a.block_rows, true);
+  CallScratch sc;
+  VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
+  pa_place(&a, lay, sc.p);
+  VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
+  VH_TRY(launch("vh_pa_delta", a.max_tiles, c.q.H, 1, 256, s, a));
+  VH_TRY(launch("vh_pa_rows_dq", a.max_blocks, c.q.H, 1, 256, s, a));
+  return launch("vh_pa_rows_dkdv", a.max_blocks, c.k.H, 1, 256, s, a);
+}
+
+size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t V) {
+  if (R <= 0 || V <= 0) return 0;
+  return LxScratch(R, V).total;
+}
+
+int vh_linear_cross_entropy_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                float ignore, float* loss, float* row_stats, int64_t R, int64_t D, int64_t V,
+                                void* scratch, size_t scratch_bytes, void* stream) {
+  const LxCall c{x, w, targets, nullptr, ldx, ldw, 0, 0, R, D, V, ignore, loss, row_stats, nullptr, nullptr, true, false};
+  return lx_run("vh_linear_cross_entropy_fwd", c, scratch, scratch_bytes, stream);
+}
+
+int vh_linear_cross_entropy_bwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                float ignore, const float* row_stats, const float* grad_out, float* dx, int64_t lddx,
+                                float* dw, int64_t lddw, int64_t R, int64_t D, int64_t V, void* scratch,
+                                size_t scratch_bytes, void* stream) {
+  const LxCall c{x,      w, targets, grad_out, ldx,     ldw, lddx, lddw, R, D, V, ignore, nullptr, const_cast<float*>(row_stats),
+                 dx, dw, false,   true};
+  return lx_run("vh_linear_cross_entropy_bwd", c, scratch, scratch_bytes, stream);
+}
+
+int vh_linear_cross_entropy_fwd_bwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
+                                    float ignore, const float* grad_out, float* loss, float* dx, int64_t lddx,
+                                    float* dw, int64_t lddw, int64_t R, int64_t D, int64_t V, void* scratch,
+                                    size_t scratch_bytes, void* stream) {
+  const LxCall c{x, w, targets, grad_out, ldx, ldw, lddx, lddw, R, D, V, ignore, loss, nullptr, dx, dw, true, true};
+  return lx_run("vh_linear_cross_entropy_fwd_bwd", c, scratch, scratch_bytes, stream);
+}
+
+}  // extern "C"

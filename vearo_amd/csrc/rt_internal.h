@@ -7,6 +7,8 @@
 
 #include "../../include/vearo_hip.h"
 
+struct VhErrRecord;
+
 namespace vh_rt {
 #define VH_RT_HIDDEN __attribute__((visibility("hidden")))
 // Records msg as this thread's vh_last_error() text and returns code.
@@ -27,4 +29,26 @@ VH_RT_HIDDEN void blaslt_shutdown();
 VH_RT_HIDDEN int noalloc_setup(int device);
 // That address (VH_NOALLOC_SCRATCH_BYTES bytes), or NULL before setup.
 VH_RT_HIDDEN void* noalloc_scratch(int device);
+// Launches a kernel of either code object with its argument struct (as the template in
+// runtime.cpp, which says what grids it refuses).
+VH_RT_HIDDEN int launch_args(const std::string& name, int64_t gx, int64_t gy, int64_t gz, unsigned block, hipStream_t s,
+                             void* args);
+// The device error record.
+VH_RT_HIDDEN VhErrRecord* error_record();
+// Compute units of the device.
+VH_RT_HIDDEN int cu_count();
+// VH_OK if a layout is not null, has a rank in [0, 8] and no negative dim or stride.
+VH_RT_HIDDEN int check_layout(const vh_layout* l, const char* what);
+
+// Scratch of one call: the caller's buffer, or a block of the arena that goes back
+// when the call's launches are queued.
+struct VH_RT_HIDDEN CallScratch {
+  void* p = nullptr;
+  hipStream_t s = nullptr;
+  bool owned = false;
+  ~CallScratch();
+  // Refuses NULL on a stream under capture: a captured graph would go on using the
+  // block after it has gone back.
+  int get(hipStream_t stream, void* user, size_t user_bytes, size_t need);
+};
 }  // namespace vh_rt

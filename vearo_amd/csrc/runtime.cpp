@@ -25,6 +25,7 @@
 
 extern "C" const unsigned char vh_code_object_start[];
 extern "C" const unsigned char vh_code_object_end[];
+extern "C" const unsigned char vh_packed_object_start[];
 
 namespace {
 
@@ -54,6 +55,7 @@ struct Runtime {
   int cu_count = 0;
   hipStream_t stream = nullptr;
   hipModule_t module = nullptr;
+  hipModule_t packed = nullptr;  // the packed-training operators' code object
   VhErrRecord* err = nullptr;  // device memory
   std::mutex fn_mu;
   std::unordered_map<std::string, hipFunction_t> fns;
@@ -77,7 +79,8 @@ int get_fn(const std::string& name, hipFunction_t* out) {
     return VH_OK;
   }
   hipFunction_t f = nullptr;
-  hipError_t e = hipModuleGetFunction(&f, g_rt.module, name.c_str());
+  const bool packed = !name.compare(0, 6, "vh_pa_") || !name.compare(0, 6, "vh_lx_") || !name.compare(0, 8, "vh_rope_");
+  hipError_t e = hipModuleGetFunction(&f, packed ? g_rt.packed : g_rt.module, name.c_str());
   if (e != hipSuccess)
     return fail(VH_ERR_HIP, "kernel " + name + " not found in code object: " + hipGetErrorString(e));
   g_rt.fns.emplace(name, f);
@@ -88,17 +91,22 @@ int get_fn(const std::string& name, hipFunction_t* out) {
 // Grid sizes arrive as 64-bit counts so that none is narrowed on the way: a
 // launch whose x dimension reaches 2^32 work-items (the dispatch packet's
 // limit), or whose y / z exceed 32 bits, is refused rather than truncated.
-template <typename A>
-int launch(const std::string& name, int64_t gx, int64_t gy, unsigned block, unsigned shmem,
-           hipStream_t s, A args, int64_t gz = 1) {
+int launch_raw(const std::string& name, int64_t gx, int64_t gy, int64_t gz, unsigned block, unsigned shmem, hipStream_t s,
+               void* args) {
   if (gx <= 0 || gy <= 0 || gz <= 0) return VH_OK;
   if (gx * (int64_t)block > (int64_t)UINT32_MAX || gy > (int64_t)UINT32_MAX || gz > (int64_t)UINT32_MAX)
     return fail(VH_ERR_UNSUPPORTED, "kernel " + name + ": grid too large for one launch");
   hipFunction_t f;
   VH_TRY(get_fn(name, &f));
-  void* params[] = {&args};
+  void* params[] = {args};
   VH_HIP(hipModuleLaunchKernel(f, (unsigned)gx, (unsigned)gy, (unsigned)gz, block, 1, 1, shmem, s, params, nullptr));
   return VH_OK;
+}
+
+template <typename A>
+int launch(const std::string& name, int64_t gx, int64_t gy, unsigned block, unsigned shmem, hipStream_t s, A args,
+           int64_t gz = 1) {
+  return launch_raw(name, gx, gy, gz, block, shmem, s, &args);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -323,8 +331,8 @@ int check_error_record() {
   VhErrRecord h;
   VH_HIP(hipStreamSynchronize(g_rt.stream));
   VH_HIP(hipMemcpy(&h, g_rt.err, sizeof h, hipMemcpyDeviceToHost));
-  if (h.token == VH_ERR_NONE && h.target == VH_ERR_NONE) return VH_OK;
-  VhErrRecord clean{VH_ERR_NONE, VH_ERR_NONE, 0, 0};
+  if (h.token == VH_ERR_NONE && h.target == VH_ERR_NONE && h.start == VH_ERR_NONE) return VH_OK;
+  VhErrRecord clean{VH_ERR_NONE, VH_ERR_NONE, 0, 0, VH_ERR_NONE, 0};
   VH_HIP(hipMemcpy(g_rt.err, &clean, sizeof clean, hipMemcpyHostToDevice));
   auto value_of = [](unsigned long long packed) {
     uint32_t bits = (uint32_t)(packed & 0xFFFFFFFFu);
@@ -338,6 +346,10 @@ int check_error_record() {
     return fail(VH_ERR_DEVICE_PANIC, "Token ID " + std::to_string(round_usize(v)) +
                                          " out of vocabulary bound " + std::to_string(h.token_bound));
   }
+  if (h.target == VH_ERR_NONE)
+    return fail(VH_ERR_DEVICE_PANIC, "Sequence start " + std::to_string((int32_t)(uint32_t)h.start) + " at index " +
+                                         std::to_string(h.start >> 32) + " is negative, before the one it follows or past the " +
+                                         std::to_string(h.start_bound) + " packed tokens");
   const float v = value_of(h.target);
   if (!(v >= 0.0f)) return fail(VH_ERR_DEVICE_PANIC, "Target class cannot be negative: " + fmt_f32(v));
   return fail(VH_ERR_DEVICE_PANIC, "Target class " + std::to_string(round_usize(v)) +
@@ -385,6 +397,33 @@ namespace vh_rt {
 int fail(int code, const std::string& msg) { return ::fail(code, msg); }
 int require_init() { return ::require_init(); }
 hipStream_t stream_of(void* s) { return S(s); }
+int launch_args(const std::string& name, int64_t gx, int64_t gy, int64_t gz, unsigned block, hipStream_t s, void* args) {
+  return launch_raw(name, gx, gy, gz, block, 0, s, args);
+}
+VhErrRecord* error_record() { return g_rt.err; }
+int cu_count() { return g_rt.cu_count; }
+int check_layout(const vh_layout* l, const char* what) { return ::check_layout(l, what); }
+CallScratch::~CallScratch() {
+  if (owned && p) g_arena.free(p, s);
+}
+int CallScratch::get(hipStream_t stream, void* user, size_t user_bytes, size_t need) {
+  s = stream;
+  if (user) {
+    if (user_bytes < need)
+      return ::fail(VH_ERR_INVALID, "scratch buffer too small: need " + std::to_string(need) + " bytes, got " +
+                                        std::to_string(user_bytes));
+    if (!aligned16(user)) return ::fail(VH_ERR_INVALID, "scratch buffer must be 16-byte aligned");
+    p = user;
+    return VH_OK;
+  }
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  VH_HIP(hipStreamIsCapturing(s, &cap));
+  if (cap != hipStreamCaptureStatusNone)
+    return ::fail(VH_ERR_INVALID, "a call under graph capture must be given its scratch buffer");
+  VH_TRY(g_arena.alloc(need, s, &p));
+  owned = true;
+  return VH_OK;
+}
 }  // namespace vh_rt
 
 // ===================================================================== ABI ==
@@ -411,10 +450,11 @@ int vh_init(int device) {
   VH_HIP(hipDeviceGetAttribute(&g_rt.cu_count, hipDeviceAttributeMultiprocessorCount, device));
   VH_HIP(hipStreamCreateWithFlags(&g_rt.stream, hipStreamNonBlocking));
   VH_HIP(hipModuleLoadData(&g_rt.module, vh_code_object_start));
+  VH_HIP(hipModuleLoadData(&g_rt.packed, vh_packed_object_start));
   void* e = nullptr;
   VH_HIP(hipMalloc(&e, sizeof(VhErrRecord)));
   g_rt.err = static_cast<VhErrRecord*>(e);
-  VhErrRecord clean{VH_ERR_NONE, VH_ERR_NONE, 0, 0};
+  VhErrRecord clean{VH_ERR_NONE, VH_ERR_NONE, 0, 0, VH_ERR_NONE, 0};
   VH_HIP(hipMemcpy(g_rt.err, &clean, sizeof clean, hipMemcpyHostToDevice));
   VH_TRY(vh_rt::noalloc_setup(device));
   g_rt.device = device;
@@ -438,6 +478,7 @@ int vh_shutdown(void) {
   }
   VH_HIP(hipFree(g_rt.err));
   VH_HIP(hipModuleUnload(g_rt.module));
+  VH_HIP(hipModuleUnload(g_rt.packed));
   VH_HIP(hipStreamDestroy(g_rt.stream));
   g_rt.fns.clear();
   g_rt.ready = false;

@@ -16,6 +16,8 @@ struct VhErrRecord {
   unsigned long long target;  // cross-entropy fwd/bwd: bad target class
   unsigned int token_bound;   // vocabulary size of the failing embedding launch
   unsigned int target_bound;  // vocabulary size of the failing cross-entropy launch
+  unsigned long long start;   // packed attention: bad sequence start (index << 32 | its int32 value)
+  unsigned int start_bound;   // packed tokens of the failing launch
 };
 #define VH_ERR_NONE 0xFFFFFFFFFFFFFFFFull
 
@@ -424,4 +426,91 @@ struct AttnDecideArgs {
   double scale;  // the attention's 1/sqrt(Dk) as f32, widened
   int32_t Dk;
   int32_t has_g;  // the backward's output gradient was probed (segment 4)
+};
+
+// Norm of queries and keys per head with the rotation by position (kernels/rope.h).
+// Tensor 0 is q, 1 is k; element (t, h, d) of x[i] is x[i][t * xt[i] + h * xh[i] + d].
+#define VH_ROPE_MAX_D 256
+struct RopeArgs {
+  const float* x[2];
+  const float* w[2];
+  const float* dy[2];  // backward
+  float* y[2];         // forward: the result; backward: dx
+  int64_t xt[2], xh[2], dt[2], dh[2], yt[2], yh[2];
+  int32_t H[2];
+  const float* positions;
+  float* part;  // backward: [workgroups][2][D] weight gradient partials
+  int64_t T;
+  int32_t D, R;         // head size, rotated elements of it
+  int32_t interleaved;  // pairs (2i, 2i + 1) instead of (i, i + R/2)
+  int32_t heads_per;    // forward: heads (of q and k in a row) per workgroup row y
+  float eps;
+  double rate[VH_ROPE_MAX_D / 2];  // half turns per position of pair i: base^(-2i/R) / pi
+};
+
+// Attention over packed sequences (kernels/packed.h).
+#define VH_PA_MAX_D 256
+// Workspace header, then the tables. A tile is 64 tokens of one sequence, a block
+// the rows one workgroup of the matrix kernels owns.
+struct PaHead {
+  int32_t ntiles, nblocks;
+  int32_t pad[2];
+};
+struct PaSpan {  // one tile or block
+  int32_t start, len;  // its sequence's first token and length
+  int32_t row0;        // its first row in the sequence
+  int32_t tile0;       // the sequence's first tile
+};
+struct PaTensor {
+  const float* p;
+  int64_t st, sh;   // strides of tokens and heads
+  int32_t H;
+  int32_t vec;      // rows may be read as 16-byte units
+};
+struct PaArgs {
+  PaTensor q, k, v, o, g;  // g: the output's gradient
+  float* out;              // forward
+  int64_t out_t, out_h;
+  float* lse;              // [Hq][T]
+  float* dq;
+  float* dk;
+  float* dv;
+  int64_t dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
+  const int32_t* starts;   // [n + 1]
+  VhErrRecord* err;
+  PaHead* head;
+  PaSpan* tiles;
+  PaSpan* blocks;
+  float* delta;            // [Hq][T]: sum over d of dout * out
+  int32_t n, T, D;
+  int32_t max_tiles, max_blocks, block_rows;
+  int32_t causal;
+  float scale;
+};
+
+// Cross-entropy of a linear layer in pieces of rows (kernels/linxent.h).
+struct LxArgs {
+  float* z;              // [rows, ld] logits of the piece; the backward's become their gradient
+  const float* targets;  // of the piece
+  const float* grad_out;
+  const float* inv;      // 1 / counted rows (0 if there is none)
+  float* stats;          // of the piece: [rows][2] row max, sum of exp
+  float* row_loss;       // of the piece, or null
+  int64_t rows, ld;
+  int32_t V;
+  float ignore;
+};
+struct LxCountArgs {
+  const float* targets;
+  float* inv;
+  VhErrRecord* err;
+  int64_t R;
+  int32_t V;
+  float ignore;
+};
+struct LxLossArgs {
+  const float* row_loss;
+  const float* inv;
+  float* loss;
+  int64_t R;
 };
