@@ -3,6 +3,7 @@
 // sequences, cross-entropy of a linear layer). Same conventions as vearo_kernels.hip.
 #include "linxent.h"
 #include "packed.h"
+#include "packed_mm.h"
 #include "rope.h"
 
 // Query / key norm and rotation: vh_rope_{fwd,bwd}_v<VW>_l<lanes per row>_n<slots per lane>
@@ -17,6 +18,13 @@ extern "C" __global__ void __launch_bounds__(256) vh_pa_delta(PaArgs a) { pa_del
 extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_fwd(PaArgs a) { pa_rows_impl<0>(a); }
 extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_dq(PaArgs a) { pa_rows_impl<1>(a); }
 extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_dkdv(PaArgs a) { pa_rows_impl<2>(a); }
+// The matrix kernels, by head size padded to 32.
+#define K_PA(DP, W1, W2, W3)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(256) vh_pa_prep_##DP(PaArgs a) { pa_prep_impl<DP>(a); }               \
+  extern "C" __global__ void __launch_bounds__(256, W1) vh_pa_fwd_##DP(PaArgs a) { pa_mm_fwd_impl<DP, 4>(a); }    \
+  extern "C" __global__ void __launch_bounds__(256, W2) vh_pa_dq_##DP(PaArgs a) { pa_mm_dq_impl<DP, 4>(a); }      \
+  extern "C" __global__ void __launch_bounds__(256, W3) vh_pa_dkdv_##DP(PaArgs a) { pa_mm_dkdv_impl<DP, 4>(a); }
+K_PA(32, 2, 2, 2) K_PA(64, 2, 2, 2) K_PA(96, 1, 1, 1) K_PA(128, 1, 1, 1)
 
 // Cross-entropy of a linear layer.
 extern "C" __global__ void __launch_bounds__(1024) vh_lx_count(LxCountArgs a) { lx_count_impl(a); }

@@ -117,24 +117,40 @@ void rope_out(RopeArgs* a, float* yq, const vh_layout* qol, float* yk, const vh_
 // ------------------------------------------------------------ packed attention --
 int64_t pa_units(int64_t T, int64_t n, int64_t rows) { return T / rows + n; }
 
-// The workspace, in the order its parts are laid out.
+// Head sizes up to kPaMatrixD run on the matrix kernels (padded to a multiple of 32), whose
+// workgroups own blocks of 128 rows; larger ones on the row kernels.
+constexpr int64_t kPaMatrixD = 128;
+int pa_padded(int64_t D) { return (int)(cdiv(D, 32) * 32); }
+int pa_block_rows(int64_t D) { return D <= kPaMatrixD ? 128 : 64; }
+
+// The workspace, in the order its parts are laid out. Streams: k, v, q, dout; each in
+// fragments by rows (n) and by columns (t) as far as the kernels read them.
 struct PaScratch {
-  size_t head, tiles, blocks, delta, total;
-  PaScratch(int64_t T, int64_t n, int64_t Hq, int64_t block_rows, bool backward) {
+  size_t head, tiles, blocks, delta, stat, n[4], t[4], info[4], total;
+  PaScratch(int64_t T, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, bool backward) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
       const size_t p = at;
       at += align256(bytes);
       return p;
     };
+    const size_t units = (size_t)pa_units(T, seqs, 64);
     head = take(sizeof(PaHead));
-    tiles = take(sizeof(PaSpan) * (size_t)pa_units(T, n, 64));
-    blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, n, block_rows));
+    tiles = take(sizeof(PaSpan) * units);
+    blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, seqs, pa_block_rows(D)));
     delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
+    const bool mm = D <= kPaMatrixD;
+    stat = take(mm && backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
+    for (int i = 0; i < 4; ++i) {
+      const bool used = mm && (backward || i < 2);
+      const size_t tiles_h = units * (size_t)(i < 2 ? Hk : Hq), bytes = tiles_h * 256 * (size_t)pa_padded(D);
+      n[i] = take(used && (backward || i == 0) ? bytes : 0);
+      t[i] = take(used && (backward ? i != 1 : i == 1) ? bytes : 0);
+      info[i] = take(used ? sizeof(int32_t) * tiles_h : 0);
+    }
     total = at;
   }
 };
-constexpr int kPaBlockRows = 64;
 
 PaTensor pa_tensor(const float* p, const vh_layout* l) {
   return PaTensor{p, l->strides[0], l->strides[1], (int32_t)l->dims[1], rows16(p, l) ? 1 : 0};
@@ -174,7 +190,7 @@ int pa_check(const std::string& f, const float* q, const vh_layout* ql, const fl
   a.n = (int32_t)n;
   a.T = (int32_t)T;
   a.D = (int32_t)D;
-  a.block_rows = kPaBlockRows;
+  a.block_rows = pa_block_rows(D);
   a.max_tiles = (int32_t)std::min<int64_t>(pa_units(T, n, 64), INT32_MAX);
   a.max_blocks = (int32_t)std::min<int64_t>(pa_units(T, n, a.block_rows), INT32_MAX);
   a.causal = causal != 0;
@@ -182,12 +198,32 @@ int pa_check(const std::string& f, const float* q, const vh_layout* ql, const fl
   return VH_OK;
 }
 
-void pa_place(PaArgs* a, const PaScratch& l, void* base) {
+// Places the workspace and, for the matrix kernels, launches the prepare step: the
+// tables and the streams' fragments.
+int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStream_t s) {
+  PaArgs& a = c->a;
   char* p = static_cast<char*>(base);
-  a->head = reinterpret_cast<PaHead*>(p + l.head);
-  a->tiles = reinterpret_cast<PaSpan*>(p + l.tiles);
-  a->blocks = reinterpret_cast<PaSpan*>(p + l.blocks);
-  a->delta = reinterpret_cast<float*>(p + l.delta);
+  a.head = reinterpret_cast<PaHead*>(p + l.head);
+  a.tiles = reinterpret_cast<PaSpan*>(p + l.tiles);
+  a.blocks = reinterpret_cast<PaSpan*>(p + l.blocks);
+  a.delta = reinterpret_cast<float*>(p + l.delta);
+  a.stat = reinterpret_cast<float*>(p + l.stat);
+  a.grad = -1;
+  if (c->q.D > kPaMatrixD) {
+    VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
+    return backward ? launch("vh_pa_delta", a.max_tiles, c->q.H, 1, 256, s, a) : VH_OK;
+  }
+  const PaTensor t[4] = {a.k, a.v, a.q, a.g};
+  const int streams = backward ? 4 : 2;
+  for (int i = 0; i < streams; ++i) {
+    const bool by_rows = backward || i == 0, by_cols = backward ? i != 1 : i == 1;
+    a.stream[i] = PaStream{t[i], by_rows ? reinterpret_cast<uint16_t*>(p + l.n[i]) : nullptr,
+                           by_cols ? reinterpret_cast<uint16_t*>(p + l.t[i]) : nullptr,
+                           reinterpret_cast<int32_t*>(p + l.info[i]), i < 2 ? VH_PA_SPAN_KV : VH_PA_SPAN_Q};
+  }
+  if (backward) a.grad = 3;
+  return launch("vh_pa_prep_" + std::to_string(pa_padded(c->q.D)), a.max_tiles, backward ? c->q.H : c->k.H, streams, 256,
+                s, a);
 }
 
 // ------------------------------------------------- cross-entropy of a linear layer --
@@ -353,7 +389,7 @@ int vh_qk_norm_rope_bwd(const float* q, const vh_layout* ql, const float* k, con
 
 size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D, int backward) {
   if (T <= 0 || n <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return 0;
-  return PaScratch(T, n, Hq, kPaBlockRows, backward != 0).total;
+  return PaScratch(T, n, Hq, Hk, D, backward != 0).total;
 }
 
 int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
@@ -367,14 +403,15 @@ int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k,
   a.out = out;
   a.out_t = ol->strides[0];
   a.out_h = ol->strides[1];
+  a.out_vec = rows16(out, ol);
   a.lse = lse;
   hipStream_t s = vh_rt::stream_of(stream);
-  const PaScratch lay(c.q.T, n, c.q.H, a.block_rows, false);
+  const PaScratch lay(c.q.T, n, c.q.H, c.k.H, c.q.D, false);
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
-  pa_place(&a, lay, sc.p);
-  VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
-  return launch("vh_pa_rows_fwd", a.max_blocks, c.q.H, 1, 256, s, a);
+  VH_TRY(pa_prepare(&c, lay, sc.p, false, s));
+  if (c.q.D > kPaMatrixD) return launch("vh_pa_rows_fwd", a.max_blocks, c.q.H, 1, 256, s, a);
+  return launch("vh_pa_fwd_" + std::to_string(pa_padded(c.q.D)), a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }
 
 int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
@@ -405,15 +442,21 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
   a.dk_h = dkl->strides[1];
   a.dv_t = dvl->strides[0];
   a.dv_h = dvl->strides[1];
+  a.dq_vec = rows16(dq, dql);
+  a.dk_vec = rows16(dk, dkl);
+  a.dv_vec = rows16(dv, dvl);
   hipStream_t s = vh_rt::stream_of(stream);
-  const PaScratch lay(c.q.T, n, c.q.H, a.block_rows, true);
+  const PaScratch lay(c.q.T, n, c.q.H, c.k.H, c.q.D, true);
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
-  pa_place(&a, lay, sc.p);
-  VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
-  VH_TRY(launch("vh_pa_delta", a.max_tiles, c.q.H, 1, 256, s, a));
-  VH_TRY(launch("vh_pa_rows_dq", a.max_blocks, c.q.H, 1, 256, s, a));
-  return launch("vh_pa_rows_dkdv", a.max_blocks, c.k.H, 1, 256, s, a);
+  VH_TRY(pa_prepare(&c, lay, sc.p, true, s));
+  if (c.q.D > kPaMatrixD) {
+    VH_TRY(launch("vh_pa_rows_dq", a.max_blocks, c.q.H, 1, 256, s, a));
+    return launch("vh_pa_rows_dkdv", a.max_blocks, c.k.H, 1, 256, s, a);
+  }
+  const std::string dp = std::to_string(pa_padded(c.q.D));
+  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H, 1, 1, 256, s, a));
+  return launch("vh_pa_dq_" + dp, a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }
 
 size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t V) {

@@ -450,6 +450,8 @@ struct RopeArgs {
 
 // Attention over packed sequences (kernels/packed.h).
 #define VH_PA_MAX_D 256
+#define VH_PA_SPAN_KV 20  // powers of two that rows of a tile of K or V, of Q or dO may
+#define VH_PA_SPAN_Q 30   // differ by on the matrix kernels
 // Workspace header, then the tables. A tile is 64 tokens of one sequence, a block
 // the rows one workgroup of the matrix kernels owns.
 struct PaHead {
@@ -467,8 +469,19 @@ struct PaTensor {
   int32_t H;
   int32_t vec;      // rows may be read as 16-byte units
 };
+struct PaStream {  // a tensor that the matrix kernels stream, split by the prepare launch
+  PaTensor t;
+  uint16_t* n;      // fragments by rows and by columns, or null
+  uint16_t* tr;
+  int32_t* info;    // [tiles][H] exponents
+  int32_t span;     // rows of a tile may differ by so many powers of two
+};
 struct PaArgs {
   PaTensor q, k, v, o, g;  // g: the output's gradient
+  PaStream stream[4];      // k, v, q, g (forward: the first two)
+  int32_t grad;            // the gradient's stream (the prepare launch forms delta with it), or -1
+  int32_t out_vec, dq_vec, dk_vec, dv_vec;  // rows may be written as 16-byte units
+  float* stat;             // [tiles][Hq][2][32 log2-lse - 14, 32 delta]
   float* out;              // forward
   int64_t out_t, out_h;
   float* lse;              // [Hq][T]
