@@ -79,6 +79,29 @@ VH_DEV void pa_find(const PaArgs& a, int idx, PaFind& f, int (&tot)[2]) {
   }
 }
 
+// Where block `b` stands in the order that its workgroups are dealt out in, the costliest
+// first (a long block begun last would run on alone). Block c of a sequence costs c + 1
+// where causal (dk and dv: counted from the sequence's end), else as much as the sequence
+// has blocks.
+VH_DEV int pa_rank(const PaArgs& a, const PaSpan& b, PaFind& f) {
+  const int tid = threadIdx.x, c = b.row0 / a.block_rows, own = (b.len + a.block_rows - 1) / a.block_rows;
+  int rank = 0;
+  for (int i = tid; i < a.n; i += 256) {
+    const int s0 = a.starts[i], s1 = a.starts[i + 1];
+    if (s0 < 0 || s1 < s0 || s1 > a.T) continue;
+    const int nb = (s1 - s0 + a.block_rows - 1) / a.block_rows;
+    const bool before = s0 < b.start;
+    if (a.causal) rank += max(0, nb - c - 1) + (before && nb > c ? 1 : 0);
+    else rank += nb > own || (nb == own && before) ? nb : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) rank += __shfl_xor(rank, o, 64);
+  if ((tid & 63) == 0) f.wave[tid >> 6][0] = rank;
+  __syncthreads();
+  rank = f.wave[0][0] + f.wave[1][0] + f.wave[2][0] + f.wave[3][0];
+  return a.causal ? rank : rank + c;
+}
+
 // Writes entry blockIdx.x of the tables; workgroup 0 also the header. A bad start
 // leaves the header without tiles: the launches that follow then do nothing.
 VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
@@ -92,9 +115,11 @@ VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
   } else {
     pa_find<false>(a, idx, f, tot);
   }
-  if (threadIdx.x == 0) {
-    if (f.tile.len >= 0 && idx < a.max_tiles) a.tiles[idx] = f.tile;
-    if (f.block.len >= 0 && idx < a.max_blocks) a.blocks[idx] = f.block;
+  if (threadIdx.x == 0 && f.tile.len >= 0 && idx < a.max_tiles) a.tiles[idx] = f.tile;
+  if (f.block.len >= 0 && idx < a.max_blocks) {
+    const int at = pa_rank(a, f.block, f);
+    // (Starts out of order could rank two blocks alike: then none is used.)
+    if (threadIdx.x == 0 && at < a.max_blocks) a.blocks[at] = f.block;
   }
 }
 

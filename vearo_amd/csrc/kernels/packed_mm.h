@@ -31,6 +31,8 @@
 // registers where the second takes its operand: register r of a 32 x 32 result is
 // row 8 (r / 4) + 4 (l / 32) + r % 4, so kind T orders its 16 tokens that way.
 #pragma once
+#include <type_traits>
+
 #include "packed.h"
 
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
@@ -82,8 +84,17 @@ VH_DEV void pa_mma(const PaFrag& a, const PaFrag& b, pa_f16& c) {
 VH_DEV float pa_ldexp(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
 // floor(log2(|x|)) of a finite nonzero x.
 VH_DEV int pa_exp(float x) { return __builtin_amdgcn_frexp_expf(x) - 1; }
-// The larger of a value and the other half wave's.
-VH_DEV float pa_max_halves(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+// The larger (the sum) of a value and the other half wave's.
+VH_DEV float pa_max_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+VH_DEV float pa_sum_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // ------------------------------------------------------------------- prepare --
 // Grid: (tiles or blocks, whichever more; heads; tensors). The tensor's tile goes through
@@ -329,85 +340,67 @@ VH_DEV bool pa_slow(PaRange r) {
 }
 
 // -------------------------------------------------------------------- forward --
-// A workgroup per block of 32 NW queries and head, 32 queries a wave; keys in tiles
-// of 64 through two LDS stages. The running maximum m of a row (in log2 units, scaled) is
-// raised only when a tile's maximum passes it by more than 8, so that most tiles leave
-// the accumulators alone; P is held at 2^6 times its value against that m, below 2^14.
+// A workgroup per block of 32 NW queries and head, 32 queries a wave; keys in steps of
+// 32 through two LDS stages. A step multiplies the next step's S while its own P is formed
+// and multiplied by V: the matrix unit and the vector unit (exp is a quarter rate) have
+// about as much to do, and a wave alone would have them take turns. So K runs one step
+// ahead of V. The running maximum m of a row (in log2 units, scaled) is raised only when
+// a step's maximum passes it by more than PA_LAG, so that most steps leave the
+// accumulators alone; P is held at 2^PA_PSHIFT times its value against that m, below 2^14.
 #define PA_LAG 8.0f
 #define PA_PSHIFT 6.0f
 template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][2 * SUB], lv[2][2 * SUB];
+  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
   const int nb = a.head->nblocks, H = a.q.H, id = blockIdx.x;
   if (id >= nb * H) return;
-  const PaSpan sp = a.blocks[nb - 1 - id / H];
+  const PaSpan sp = a.blocks[id / H];
   const int h = id % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
-  const int end = min(sp.len, sp.row0 + 32 * NW);
-  const int nt = ((a.causal ? end : sp.len) + 63) >> 6;
+  const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
   PaRange rk, rv;
-  pa_scan(sk.info, a.k.H, hk, sp.tile0, sp.tile0 + nt, rk);
-  pa_scan(sv.info, a.k.H, hk, sp.tile0, sp.tile0 + nt, rv);
+  pa_scan(sk.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk);
+  pa_scan(sv.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rv);
   rv.slow |= rk.slow;
   if (pa_slow(rv)) {
     pa_rows<0>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
     return;
   }
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
-  const bool busy = r0 < sp.len;
+  const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
+  auto stage = [&](const uint16_t* p, int t, uint16_t* to) {
+    pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
+  };
+  stage(sk.n, 0, lk[0]);
+  stage(sv.tr, 0, lv[0]);
+  if (nt > 1) stage(sk.n, 1, lk[1]);
   PaFrag q[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q);
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
   const float cs = a.scale * PA_LOG2E;
-  const int64_t chunk = (int64_t)a.k.H * (2 * SUB);
-  const uint16_t* pk = sk.n + ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB);
-  const uint16_t* pv = sv.tr + ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB);
-  auto stage = [&](int t, int b) {
-    pa_copy<NW, 4 * SUB>(pk + t * chunk, lk[b]);
-    pa_copy<NW, 4 * SUB>(pv + t * chunk, lv[b]);
-  };
-  pa_f16 o[DB];
+  pa_f16 o[DB], s{};
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = pa_f16{};
   float m = -INFINITY, l = 0.0f;
   int ev = 0;
-  stage(0, 0);
-  for (int t = 0; t < nt; ++t) {
-    const int64_t it = (int64_t)(sp.tile0 + t) * a.k.H + hk;
-    const int ek = sk.info[it], evt = sv.info[it];
-    pa_arrived();
+  // Steps that some row of the wave sees.
+  const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
+  // The steps' exponents, read one step ahead.
+  const int32_t *ik = sk.info + (int64_t)sp.tile0 * a.k.H + hk, *iv = sv.info + (int64_t)sp.tile0 * a.k.H + hk;
+  int ekn = *ik, evn = *iv;
+  auto step = [&](int t, int ek, int evt, auto more) {
     const int b = t & 1;
-    if (t + 1 < nt) stage(t + 1, b ^ 1);
-    // 32-key halves of the tile that some row of the wave sees.
-    const int seen = (a.causal ? min(r0 + 32, sp.len) : sp.len) - 64 * t;
-    const int ns = !busy || seen <= 0 ? 0 : seen <= 32 ? 1 : 2;
-    if (ns == 0) continue;
-    pa_f16 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (u >= ns) break;
-      s[u] = pa_f16{};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) pa_mma(pa_frag(lk[b] + u * SUB, k, KS), q[k], s[u]);
-    }
     const float c = fmaxf(pa_ldexp(cs, eq + (ek == PA_ZERO ? 0 : ek) - 2 * PA_E), 0x1p-126f);
-    const int key0 = 64 * t + 4 * hf;
-    if (64 * t + 32 * ns > (a.causal ? r0 + 1 : sp.len)) {  // some row does not see all of it
+    if (32 * t + 32 > (a.causal ? r0 + 1 : sp.len)) {  // some row does not see all of it
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (u < ns && key0 + 32 * u + 8 * (r >> 2) + (r & 3) > lim) s[u][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (32 * t + 4 * hf + 8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
     }
-    float mt = -INFINITY;
+    float mt = s[0];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (u < ns) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[u][r]);
-      }
+    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
     mt = pa_max_halves(mt) * c;
     if (__builtin_amdgcn_ballot_w64(mt > m + PA_LAG) != 0) {
       const float mn = fmaxf(m, mt), al = __builtin_amdgcn_exp2f(m - mn);
@@ -420,23 +413,43 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
     }
     pa_units_to(evt, ev, o);
     const float ms = m - PA_PSHIFT;
+    pa_f16 next{};
+    if constexpr (decltype(more)::value) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (u >= ns) break;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -ms));
-#pragma unroll
-      for (int r = 0; r < 16; ++r) l += s[u][r];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const PaFrag p = pa_split8([&](int k) { return s[u][8 * g + k]; });
-#pragma unroll
-        for (int db = 0; db < DB; ++db) pa_mma(pa_frag(lv[b] + u * SUB, 2 * db + g, 2 * DB), p, o[db]);
-      }
+      for (int k = 0; k < KS; ++k) pa_mma(pa_frag(lk[b ^ 1], k, KS), q[k], next);
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ms));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) l += s[r];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const PaFrag p = pa_split8([&](int k) { return s[8 * g + k]; });
+#pragma unroll
+      for (int db = 0; db < DB; ++db) pa_mma(pa_frag(lv[b], 2 * db + g, 2 * DB), p, o[db]);
+    }
+    s = next;
+  };
+  // Arrived: V of step t and K of step t + 1; then V of t + 1 and K of t + 2 go out.
+  pa_arrived();
+  if (mine > 0) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) pa_mma(pa_frag(lk[0], k, KS), q[k], s);
   }
-  if (!busy) return;
-  l += __shfl_xor(l, 32, 64);
+  for (int t = 0; t < nt; ++t) {
+    if (t) pa_arrived();
+    else __syncthreads();  // (K of step 0 has been read)
+    if (t + 1 < nt) stage(sv.tr, t + 1, lv[(t + 1) & 1]);
+    if (t + 2 < nt) stage(sk.n, t + 2, lk[t & 1]);
+    const int ek = ekn, evt = evn;
+    const int64_t ahead = (int64_t)(min(t + 1, nt - 1) >> 1) * a.k.H;
+    ekn = ik[ahead];
+    evn = iv[ahead];
+    if (t + 1 < mine) step(t, ek, evt, std::true_type{});
+    else if (t < mine) step(t, ek, evt, std::false_type{});
+  }
+  if (r0 >= sp.len) return;
+  l = pa_sum_halves(l);
   if (i >= sp.len) return;
   const int64_t tok = (int64_t)sp.start + i;
   const float inv = 1.0f / l;
@@ -474,7 +487,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   __shared__ __attribute__((aligned(1024))) uint16_t ls[2][3 * SUB];  // K by rows, K by columns, V by rows
   const int nb = a.head->nblocks, H = a.q.H, id = blockIdx.x;
   if (id >= nb * H) return;
-  const PaSpan sp = a.blocks[nb - 1 - id / H];
+  const PaSpan sp = a.blocks[id / H];
   const int h = id % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const int end = min(sp.len, sp.row0 + 32 * NW);
@@ -560,7 +573,9 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   __shared__ __attribute__((aligned(1024))) float lst[2][64];
   const int nb = a.head->nblocks, H = a.k.H, id = blockIdx.x;
   if (id >= nb * H) return;
-  const PaSpan sp = a.blocks[id / H];
+  PaSpan sp = a.blocks[id / H];
+  // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
+  if (a.causal) sp.row0 = (sp.len - 1) / a.block_rows * a.block_rows - sp.row0;
   const int hk = id % H, G = a.q.H / H;
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1], &sq = a.stream[2], &sg = a.stream[3];
