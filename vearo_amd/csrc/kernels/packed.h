@@ -209,13 +209,14 @@ VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, float* l,
     if (lane + 64 * u < a.D) a.dq[tok * a.dq_t + h * a.dq_h + lane + 64 * u] = acc[u] * a.scale;
 }
 
-VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float* l, float* lv) {
-  const int lane = threadIdx.x & 63, G = a.q.H / a.k.H;
+// Over query heads h0 .. h1 - 1, into dk and dv or, of several parts, into this one's sums.
+VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float* l, float* lv, int h0, int h1, int part) {
+  const int lane = threadIdx.x & 63;
   const int64_t tok = (int64_t)sp.start + j;
   pa_row_to_lds(l, a.k.p + tok * a.k.st + hk * a.k.sh, a.D);
   pa_row_to_lds(lv, a.v.p + tok * a.v.st + hk * a.v.sh, a.D);
   float dk[4] = {}, dv[4] = {};
-  for (int h = hk * G; h < (hk + 1) * G; ++h) {
+  for (int h = h0; h < h1; ++h) {
     const float* q = a.q.p + sp.start * a.q.st + h * a.q.sh;
     const float* g = a.g.p + sp.start * a.g.st + h * a.g.sh;
     const int64_t at = (int64_t)h * a.T + sp.start;
@@ -230,23 +231,31 @@ VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float*
       pa_axpy(p, g + i0 * a.g.st, a.g.st, m, a.D, dv);
     }
   }
+  float* ok = a.dk + tok * a.dk_t + hk * a.dk_h;
+  float* ov = a.dv + tok * a.dv_t + hk * a.dv_h;
+  if (a.parts > 1) {
+    const int dp = (a.D + 31) / 32 * 32;
+    ok = a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * dp;
+    ov = ok + (int64_t)a.T * a.k.H * dp;
+  }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (lane + 64 * u < a.D) {
-      a.dk[tok * a.dk_t + hk * a.dk_h + lane + 64 * u] = dk[u] * a.scale;
-      a.dv[tok * a.dv_t + hk * a.dv_h + lane + 64 * u] = dv[u];
+      ok[lane + 64 * u] = dk[u] * a.scale;
+      ov[lane + 64 * u] = dv[u];
     }
 }
 
 // The rows of one block, over the workgroup's waves. MODE 0 forward, 1 dq, 2 dk and dv.
 template <int MODE>
-VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, float (*l)[2][VH_PA_MAX_D]) {
+VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, float (*l)[2][VH_PA_MAX_D], int h0 = 0, int h1 = 0,
+                    int part = 0) {
   const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int end = min(sp.len, sp.row0 + a.block_rows);
   for (int i = sp.row0 + w; i < end; i += nw) {
     if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l[w][0]);
     if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l[w][0], l[w][1]);
-    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l[w][0], l[w][1]);
+    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l[w][0], l[w][1], h0, h1, part);
   }
 }
 // Grid: (blocks, heads: of q, or of k for dk and dv).
@@ -254,7 +263,8 @@ template <int MODE>
 VH_DEV void pa_rows_impl(const PaArgs& a) {
   __shared__ float l[4][2][VH_PA_MAX_D];
   if ((int)blockIdx.x >= a.head->nblocks) return;
-  pa_rows<MODE>(a, blockIdx.y, a.blocks[blockIdx.x], l);
+  const int G = a.q.H / a.k.H;
+  pa_rows<MODE>(a, blockIdx.y, a.blocks[blockIdx.x], l, blockIdx.y * G, (blockIdx.y + 1) * G);
 }
 
 // delta[h][t] = sum over d of dout * out for every row of the sequences, a wave per row

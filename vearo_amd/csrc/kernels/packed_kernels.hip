@@ -23,8 +23,9 @@ extern "C" __global__ void __launch_bounds__(256) vh_pa_rows_dkdv(PaArgs a) { pa
   extern "C" __global__ void __launch_bounds__(256) vh_pa_prep_##DP(PaArgs a) { pa_prep_impl<DP>(a); }               \
   extern "C" __global__ void __launch_bounds__(256, W1) vh_pa_fwd_##DP(PaArgs a) { pa_mm_fwd_impl<DP, 4>(a); }    \
   extern "C" __global__ void __launch_bounds__(256, W2) vh_pa_dq_##DP(PaArgs a) { pa_mm_dq_impl<DP, 4>(a); }      \
-  extern "C" __global__ void __launch_bounds__(256, W3) vh_pa_dkdv_##DP(PaArgs a) { pa_mm_dkdv_impl<DP, 4>(a); }
-K_PA(32, 4, 2, 2) K_PA(64, 3, 2, 2) K_PA(96, 2, 1, 1) K_PA(128, 2, 1, 1)
+  extern "C" __global__ void __launch_bounds__(256, W3) vh_pa_dkdv_##DP(PaArgs a) { pa_mm_dkdv_impl<DP, 4>(a); }  \
+  extern "C" __global__ void __launch_bounds__(256) vh_pa_join_##DP(PaArgs a) { pa_join_impl<DP>(a); }
+K_PA(32, 4, 4, 3) K_PA(64, 3, 3, 2) K_PA(96, 2, 2, 1) K_PA(128, 2, 1, 1)
 
 // Cross-entropy of a linear layer.
 extern "C" __global__ void __launch_bounds__(1024) vh_lx_count(LxCountArgs a) { lx_count_impl(a); }

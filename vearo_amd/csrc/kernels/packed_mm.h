@@ -14,28 +14,32 @@
 //   - one that a wave holds has one per row, which is a lane there;
 //   - P is at most 1 by construction; dS takes a power of two per row (column) that
 //     is lowered when a tile's largest needs it, as the softmax's running maximum is.
-// Accumulators are in the units of the running tile scale and are multiplied over when
-// it changes (exact). A tile whose rows differ by more than VH_PA_SPAN_KV (K, V) or
+// A sum over tiles is in the units of one of them: what a tile's power of two differs by
+// goes into the other operand (into dS's own scale; into P's while it is within
+// PA_SHIFT, beyond which the accumulators are multiplied over, exactly). A tile whose rows differ by more than VH_PA_SPAN_KV (K, V) or
 // VH_VH_PA_SPAN_Q (Q, dO) powers of two, tiles of one stream that differ by more than
 // PA_SPAN_TILES, and infinities and NaN send the workgroup's block to the row kernels of
 // packed.h, which have no such limits.
 //
 // A first launch (pa_prep) splits the streamed tensors once, into the order the
-// matrix instruction's lanes take them: a fragment is 64 lanes x 16 bytes. The main
-// kernels copy fragments into LDS as they lie (no registers, no bank conflicts) and
-// read them back 16 bytes a lane. Fragments of kind N hold 32 tokens x 16 elements
-// (lane l: token l % 32, elements 8 (l / 32) ..), for products over the head's
-// elements; kind T holds 32 elements x 16 tokens, for products over tokens. A wave
-// computes S with its own rows as the columns of the result, so a row's softmax
+// matrix instruction's lanes take them: a fragment is 32 tokens x 16 elements of one part,
+// 64 pieces of 16 bytes, piece (hh, t) the elements 8 hh .. 8 hh + 7 of token t. The main
+// kernels copy fragments into LDS as they lie (no registers) and read them two ways:
+// by rows, a piece a lane (products over the head's elements: S, dO V^T), and by
+// columns with the transposing LDS read (products over tokens). Pieces lie at
+// 32 hh + (t ^ 4 hh ^ 8 (k & 1)) of fragment k, which keeps both free of bank conflicts.
+// A wave computes S with its own rows as the columns of the result, so a row's softmax
 // statistics are lane scalars, and P and dS leave the first product in exactly the
 // registers where the second takes its operand: register r of a 32 x 32 result is
-// row 8 (r / 4) + 4 (l / 32) + r % 4, so kind T orders its 16 tokens that way.
+// row 8 (r / 4) + 4 (l / 32) + r % 4, and the column reads take tokens in that order.
 #pragma once
 #include <type_traits>
 
 #include "packed.h"
 
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pa_h4 __attribute__((ext_vector_type(4)));
+typedef short pa_s4 __attribute__((ext_vector_type(4)));
 typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
 typedef float pa_f2 __attribute__((ext_vector_type(2)));
 typedef float pa_f4 __attribute__((ext_vector_type(4)));
@@ -46,6 +50,8 @@ typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
 #define PA_ZERO 1000       // tile exponents: all zero; not for the matrix kernels
 #define PA_SLOW 2000
 #define PA_SPAN_TILES 60
+#define PA_SHIFT 3
+#define PA_PV 11           // dV's P is held at 2^11, below 2^14 with the shift
 #define PA_LOG2E 1.4426950408889634f
 #define PA_LN2 0.6931471805599453f
 
@@ -96,12 +102,14 @@ VH_DEV float pa_sum_halves(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Where lane l's piece (hh = l / 32, t = l % 32) of fragment k lies in it.
+VH_DEV int pa_piece(int l, int k) { return l ^ (l >> 5 << 2) ^ ((k & 1) << 3); }
+
 // ------------------------------------------------------------------- prepare --
 // Grid: (tiles or blocks, whichever more; heads; tensors). The tensor's tile goes through
-// LDS once and out as fragments of the kinds asked for. The gradient's workgroups also
-// write delta and, per tile, what dk/dv reads per query: log2-lse - PA_E and delta, 32
+// LDS once and out as fragments. The gradient's workgroups also
+// write delta and, per tile, what dk/dv reads per query: log2-lse - PA_PV and delta, 32
 // rows of each at a time, +inf and 0 past the sequence.
-// Floats of a fragment tile: 2 parts x 64 tokens x DP.
 template <int DP>
 VH_DEV void pa_prep_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, LD = DP + 4;
@@ -160,7 +168,7 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
     const int64_t tok = (int64_t)h * a.T + sp.start + i;
     if ((tid & 3) == 0) {
       float* s = a.stat + at * 128 + (row >> 5) * 64 + (row & 31);
-      s[0] = live ? a.lse[tok] * PA_LOG2E - (float)PA_E : INFINITY;
+      s[0] = live ? a.lse[tok] * PA_LOG2E - (float)PA_PV : INFINITY;
       s[32] = live ? dl : 0.0f;
       if (live) a.delta[tok] = dl;
     }
@@ -190,25 +198,15 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
   }
   if (tid == 0) st.info[at] = info;
   if (info == PA_SLOW) return;  // (its fragments are never used)
-  auto put = [&](uint16_t* base, int sub, int frag, int nfrag, const PaFrag& v) {
-    pa_u4* q = reinterpret_cast<pa_u4*>(base + at * (128 * DP) + sub * (64 * DP)) + frag * 64 + lane;
-    q[0] = __builtin_bit_cast(pa_u4, v.h);
-    q[nfrag * 64] = __builtin_bit_cast(pa_u4, v.l);
-  };
   const int li = lane & 31, hf = lane >> 5;
-  if (st.n) {  // [sub-tile of 32 tokens][part][16 elements]
-    for (int u = w; u < 2 * KS; u += 4) {
-      const float* q = &x[(32 * (u / KS) + li) * LD + 16 * (u % KS) + 8 * hf];
-      put(st.n, u / KS, u % KS, KS, pa_split8([&](int k) { return pa_ldexp(q[k], PA_E - e); }));
-    }
-  }
-  if (st.tr) {  // [sub-tile][part][32 elements][16 tokens]
-    for (int u = w; u < 4 * DB; u += 4) {
-      const int sub = u / (2 * DB), db = (u >> 1) % DB, s = u & 1;
-      const float* q = &x[(32 * sub + 16 * s + 4 * hf) * LD + 32 * db + li];
-      put(st.tr, sub, db * 2 + s, 2 * DB,
-          pa_split8([&](int k) { return pa_ldexp(q[(8 * (k >> 2) + (k & 3)) * LD], PA_E - e); }));
-    }
+  // [32 tokens][part][16 elements][piece]
+  for (int u = w; u < 2 * KS; u += 4) {
+    const int sub = u / KS, k = u % KS;
+    const float* q = &x[(32 * sub + li) * LD + 16 * k + 8 * hf];
+    const PaFrag v = pa_split8([&](int j) { return pa_ldexp(q[j], PA_E - e); });
+    pa_u4* to = reinterpret_cast<pa_u4*>(st.n + at * (128 * DP) + sub * (64 * DP)) + k * 64 + pa_piece(lane, k);
+    to[0] = __builtin_bit_cast(pa_u4, v.h);
+    to[KS * 64] = __builtin_bit_cast(pa_u4, v.l);
   }
 }
 
@@ -237,10 +235,38 @@ VH_DEV void pa_arrived() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
 }
-VH_DEV PaFrag pa_frag(const uint16_t* l, int frag, int nfrag) {
-  const uint16_t* p = l + frag * 512 + (threadIdx.x & 63) * 8;
-  return {*reinterpret_cast<const pa_h8*>(p), *reinterpret_cast<const pa_h8*>(p + nfrag * 512)};
-}
+// What a wave reads of a 32-token stage, 64 DP halves: [part][16 elements][piece].
+template <int DP>
+struct PaStage {
+  const uint16_t* base;
+  int row, col;  // the lane's offset in a fragment by rows (k even), by columns (first four tokens)
+  VH_DEV PaStage(const uint16_t* b) : base(b) {
+    const int l = threadIdx.x & 63;
+    row = pa_piece(l, 0) * 8;
+    // The transposing read: lanes 4 k + c of 16 give token k's elements 4 c .. 4 c + 3
+    // and lane i gets element i of the four tokens.
+    const int i = l & 15, odd = l >> 4 & 1, k = i >> 2, c = i & 3;
+    col = odd * 512 + pa_piece((c >> 1) * 32 + (l >> 5) * 4 + k, odd) * 8 + (c & 1) * 4;
+  }
+  // Tokens by rows: elements 16 k .. 16 k + 15 of the 32 tokens.
+  VH_DEV PaFrag rows(int st, int k) const {
+    const uint16_t* p = base + st * (64 * DP) + k * 512 + (k & 1 ? row ^ 64 : row);
+    return {*reinterpret_cast<const pa_h8*>(p), *reinterpret_cast<const pa_h8*>(p + DP / 16 * 512)};
+  }
+  // Elements 32 db .. 32 db + 31 by rows, of 16 tokens: 8 (p / 4) + 4 (l / 32) + p % 4 past 16 u.
+  VH_DEV PaFrag cols(int st, int db, int u) const {
+    const uint16_t* p = base + st * (64 * DP) + db * 1024 + u * 128;
+    auto four = [](const uint16_t* q) {
+      return __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) pa_s4*)const_cast<uint16_t*>(q)));
+    };
+    auto eight = [&](const uint16_t* q) {
+      const pa_h4 a = four(q + col), b = four(q + (col ^ 64));
+      return pa_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    };
+    return {eight(p), eight(p + DP / 16 * 512)};
+  }
+};
 
 // A wave's own 32 rows of a tensor as operand fragments: lane l holds row r0 + l % 32,
 // scaled by its own power of two; returns the exponent (0 for a row of zeros or past
@@ -301,17 +327,19 @@ VH_DEV void pa_store(float* p, bool vec, int D, const pa_f16 (&acc)[DB], F value
     }
 }
 
-// Running accumulator scale of a streamed tensor's tiles: brings acc to exponent e's
-// units. `cur` is the exponent its units are in now.
+// What a tile of exponent e differs by from the accumulators' units `cur`; beyond
+// PA_SHIFT the accumulators are brought to e's.
 template <int DB>
-VH_DEV void pa_units_to(int e, int& cur, pa_f16 (&acc)[DB]) {
-  if (e == cur || e == PA_ZERO) return;
+VH_DEV int pa_shift(int e, int& cur, pa_f16 (&acc)[DB]) {
+  if (e == PA_ZERO) return 0;
+  if (e - cur >= -PA_SHIFT && e - cur <= PA_SHIFT) return e - cur;
   const float s = pa_ldexp(1.0f, cur - e);
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] *= s;
   cur = e;
+  return 0;
 }
 
 // Looks over the exponents of tiles t0 .. t1 - 1 of a stream: whether one is not for the
@@ -330,13 +358,16 @@ VH_DEV void pa_scan(const int32_t* info, int64_t H, int h, int t0, int t1, PaRan
     }
   }
 }
-VH_DEV bool pa_slow(PaRange r) {
+VH_DEV bool pa_slow(PaRange& r) {
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
     r.lo = min(r.lo, __shfl_xor(r.lo, k, 64));
     r.hi = max(r.hi, __shfl_xor(r.hi, k, 64));
   }
-  return __builtin_amdgcn_ballot_w64(r.slow) != 0 || r.hi - r.lo > PA_SPAN_TILES;
+  r.hi = __builtin_amdgcn_readfirstlane(r.hi);
+  const bool slow = __builtin_amdgcn_ballot_w64(r.slow) != 0 || r.hi - r.lo > PA_SPAN_TILES;
+  if (r.hi < -1000) r.hi = 0;  // (zeros only)
+  return slow;
 }
 
 // -------------------------------------------------------------------- forward --
@@ -348,7 +379,7 @@ VH_DEV bool pa_slow(PaRange r) {
 // a step's maximum passes it by more than PA_LAG, so that most steps leave the
 // accumulators alone; P is held at 2^PA_PSHIFT times its value against that m, below 2^14.
 #define PA_LAG 8.0f
-#define PA_PSHIFT 6.0f
+#define PA_PSHIFT 3.0f
 template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
@@ -368,13 +399,14 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
     pa_rows<0>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
     return;
   }
+  const PaStage<DP> fk(lk[0]), fv(lv[0]);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
   const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
   auto stage = [&](const uint16_t* p, int t, uint16_t* to) {
     pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
   };
   stage(sk.n, 0, lk[0]);
-  stage(sv.tr, 0, lv[0]);
+  stage(sv.n, 0, lv[0]);
   if (nt > 1) stage(sk.n, 1, lk[1]);
   PaFrag q[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q);
@@ -411,22 +443,24 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= al;
     }
-    pa_units_to(evt, ev, o);
-    const float ms = m - PA_PSHIFT;
+    const int sh = pa_shift(evt, ev, o);
+    const float ms = m - PA_PSHIFT - (float)sh;
     pa_f16 next{};
     if constexpr (decltype(more)::value) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) pa_mma(pa_frag(lk[b ^ 1], k, KS), q[k], next);
+      for (int k = 0; k < KS; ++k) pa_mma(fk.rows(b ^ 1, k), q[k], next);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ms));
+    float ls = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) l += s[r];
+    for (int r = 0; r < 16; ++r) ls += s[r];
+    l = fmaf(ls, pa_ldexp(1.0f, -sh), l);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const PaFrag p = pa_split8([&](int k) { return s[8 * g + k]; });
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(pa_frag(lv[b], 2 * db + g, 2 * DB), p, o[db]);
+      for (int db = 0; db < DB; ++db) pa_mma(fv.cols(b, db, g), p, o[db]);
     }
     s = next;
   };
@@ -434,12 +468,12 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   pa_arrived();
   if (mine > 0) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) pa_mma(pa_frag(lk[0], k, KS), q[k], s);
+    for (int k = 0; k < KS; ++k) pa_mma(fk.rows(0, k), q[k], s);
   }
   for (int t = 0; t < nt; ++t) {
     if (t) pa_arrived();
     else __syncthreads();  // (K of step 0 has been read)
-    if (t + 1 < nt) stage(sv.tr, t + 1, lv[(t + 1) & 1]);
+    if (t + 1 < nt) stage(sv.n, t + 1, lv[(t + 1) & 1]);
     if (t + 2 < nt) stage(sk.n, t + 2, lk[t & 1]);
     const int ek = ekn, evt = evn;
     const int64_t ahead = (int64_t)(min(t + 1, nt - 1) >> 1) * a.k.H;
@@ -459,50 +493,60 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
 }
 
 // -------------------------------------------------------------------- backward --
-// dS under its running power of two: bring 2^g up to where the largest |dS| of the
-// tile stays below 2^15, and the accumulators with it, only where it does not already.
+// dS under its running power of two 2^g: returns what to multiply dS by, 2^(g + sh)
+// where sh is the tile's difference from the accumulators' units, after lowering g (and
+// multiplying the accumulators over) where the tile's largest would pass 2^15.
 template <int DB>
-VH_DEV void pa_fit(const pa_f16& ds, float& gs, int& g, pa_f16 (&acc)[DB]) {
+VH_DEV float pa_fit(const pa_f16& ds, int sh, int& g, pa_f16 (&acc)[DB]) {
   float mx = 0.0f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) mx = fmaxf(mx, fabsf(ds[r]));
   mx = pa_max_halves(mx);
-  const bool over = mx * gs > 32768.0f;
-  if (__builtin_amdgcn_ballot_w64(over) == 0) return;
-  const int gn = over ? max(min(10 - pa_exp(mx), 126), -126) : g;
-  const float f = pa_ldexp(1.0f, gn - g);
+  float f = pa_ldexp(1.0f, g + sh);
+  const bool over = mx * f > 32768.0f;
+  if (__builtin_amdgcn_ballot_w64(over) == 0) return f;
+  const int gn = over ? max(min(10 - pa_exp(mx) - sh, 126), -126) : g;
+  const float s = pa_ldexp(1.0f, gn - g);
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[db][r] *= f;
+    for (int r = 0; r < 16; ++r) acc[db][r] *= s;
   g = gn;
-  gs = pa_ldexp(1.0f, g);
+  return pa_ldexp(1.0f, g + sh);
 }
 
-// dq: as the forward, with dO beside Q, in steps of 32 keys; S and dO V^T of the step,
-// dS, then dS K.
+// dq: as the forward, with dO beside Q: S, then dO V^T under the exp of S, then dS K from
+// the same stage of K, read by columns. (The next step's products under this one's, as in
+// the forward, hold 32 registers more and a third stage of K: measured slower, 145 against
+// 125 us for 16384 tokens of 40 sequences, 12 heads of 64, at two waves a SIMD for three.)
 template <int DP, int NW>
 VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  __shared__ __attribute__((aligned(1024))) uint16_t ls[2][3 * SUB];  // K by rows, K by columns, V by rows
+  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
   const int nb = a.head->nblocks, H = a.q.H, id = blockIdx.x;
   if (id >= nb * H) return;
   const PaSpan sp = a.blocks[id / H];
   const int h = id % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
-  const int end = min(sp.len, sp.row0 + 32 * NW);
-  const int nt = ((a.causal ? end : sp.len) + 31) >> 5;
+  const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
   PaRange rk, rv;
   pa_scan(sk.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk);
   pa_scan(sv.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rv);
   rk.slow |= rv.slow;
   if (pa_slow(rk)) {
-    pa_rows<1>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&ls[0][0]));
+    pa_rows<1>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
     return;
   }
+  const PaStage<DP> fk(lk[0]), fv(lv[0]);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
-  const bool busy = r0 < sp.len, live = i < sp.len;
+  const bool live = i < sp.len;
+  const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
+  auto stage = [&](const uint16_t* p, int t, uint16_t* to) {
+    pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
+  };
+  stage(sk.n, 0, lk[0]);
+  stage(sv.n, 0, lv[0]);
   PaFrag q[KS], gq[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q), eg = pa_own<DP>(a.g, sp, a.D, i, h, gq);
   const int64_t tok = (int64_t)sp.start + i;
@@ -510,161 +554,203 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   const float dl = live ? a.delta[(int64_t)h * a.T + tok] : 0.0f;
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
   const float cs = a.scale * PA_LOG2E;
-  const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
-  auto stage = [&](int t, int b) {
-    const int64_t at = base + (t >> 1) * chunk + (t & 1) * SUB;
-    pa_copy<NW, 2 * SUB>(sk.n + at, ls[b]);
-    pa_copy<NW, 2 * SUB>(sk.tr + at, ls[b] + SUB);
-    pa_copy<NW, 2 * SUB>(sv.n + at, ls[b] + 2 * SUB);
-  };
   pa_f16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = pa_f16{};
-  int ekc = 0, g = 126;
-  float gs = 0x1p126f;
-  stage(0, 0);
+  int g = 126;
+  const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
+  const int32_t *ik = sk.info + (int64_t)sp.tile0 * a.k.H + hk, *iv = sv.info + (int64_t)sp.tile0 * a.k.H + hk;
+  int ekn = *ik, evn = *iv;
   for (int t = 0; t < nt; ++t) {
-    const int64_t it = (int64_t)(sp.tile0 + (t >> 1)) * a.k.H + hk;
-    const int ek = sk.info[it], ev = sv.info[it];
     pa_arrived();
-    const int b = t & 1;
-    if (t + 1 < nt) stage(t + 1, b ^ 1);
-    if (!busy || (a.causal && 32 * t > r0 + 31)) continue;
+    const int b = t & 1, ek = ekn, ev = evn;
+    if (t + 1 < nt) {
+      stage(sk.n, t + 1, lk[b ^ 1]);
+      stage(sv.n, t + 1, lv[b ^ 1]);
+      const int64_t ahead = (int64_t)((t + 1) >> 1) * a.k.H;
+      ekn = ik[ahead];
+      evn = iv[ahead];
+    }
+    if (t >= mine) continue;
     pa_f16 s{}, dp{};
 #pragma unroll
-    for (int k = 0; k < KS; ++k) pa_mma(pa_frag(ls[b], k, KS), q[k], s);
-#pragma unroll
-    for (int k = 0; k < KS; ++k) pa_mma(pa_frag(ls[b] + 2 * SUB, k, KS), gq[k], dp);
-    const float c = pa_ldexp(cs, eq + (ek == PA_ZERO ? 0 : ek) - 2 * PA_E);
-    const float cg = pa_ldexp(1.0f, eg + (ev == PA_ZERO ? 0 : ev) - 2 * PA_E);
-    const bool part = 32 * t + 32 > (a.causal ? r0 + 1 : sp.len);
-    const int key0 = 32 * t + 4 * hf;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
-      s[r] = p * fmaf(dp[r], cg, -dl);
-    }
-    if (part) {
+    for (int k = 0; k < KS; ++k) pa_mma(fk.rows(b, k), q[k], s);
+    if (32 * t + 32 > (a.causal ? r0 + 1 : sp.len)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (key0 + 8 * (r >> 2) + (r & 3) > lim) s[r] = 0.0f;
+        if (32 * t + 4 * hf + 8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
     }
-    pa_units_to(ek, ekc, acc);
-    pa_fit(s, gs, g, acc);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) pa_mma(fv.rows(b, k), gq[k], dp);
+    const float c = fmaxf(pa_ldexp(cs, eq + (ek == PA_ZERO ? 0 : ek) - 2 * PA_E), 0x1p-126f);
+    const float cg = pa_ldexp(1.0f, eg + (ev == PA_ZERO ? 0 : ev) - 2 * PA_E);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= fmaf(dp[r], cg, -dl);
+    const float gs = pa_fit(s, ek == PA_ZERO ? 0 : ek - rk.hi, g, acc);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const PaFrag f = pa_split8([&](int k) { return s[8 * u + k] * gs; });
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(pa_frag(ls[b] + SUB, 2 * db + u, 2 * DB), f, acc[db]);
+      for (int db = 0; db < DB; ++db) pa_mma(fk.cols(b, db, u), f, acc[db]);
     }
   }
   if (!live) return;
   pa_store<DB>(a.dq + tok * a.dq_t + h * a.dq_h, a.dq_vec, a.D, acc,
-               [&](float v) { return pa_ldexp(v * a.scale, ekc - PA_E - g); });
+               [&](float v) { return pa_ldexp(v * a.scale, rk.hi - PA_E - g); });
 }
 
-// dk and dv: a workgroup per block of 32 NW keys and key head, 32 keys a wave, over
-// the queries that see them, 32 at a time, of every query head of the key head.
+// dk and dv: a workgroup per block of 32 NW keys, key head and part of its query heads,
+// 32 keys a wave, over the queries that see them, 32 at a time; Q and dO are read by
+// rows for S and dO V^T and by columns for dV and dK. Its accumulators and resident rows
+// leave no registers for a second step's S: what overlaps is the exp of S with dO V^T and
+// dS with dV. Where the blocks are few the query heads are divided over a.parts workgroups,
+// whose sums pa_join adds in order.
 template <int DP, int NW>
 VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  // Q by rows, Q by columns, dO by rows, dO by columns; 32 log2-lse and 32 delta.
-  __shared__ __attribute__((aligned(1024))) uint16_t ls[2][4 * SUB];
-  __shared__ __attribute__((aligned(1024))) float lst[2][64];
-  const int nb = a.head->nblocks, H = a.k.H, id = blockIdx.x;
+  __shared__ __attribute__((aligned(1024))) uint16_t lq[2][SUB], lg[2][SUB];
+  __shared__ __attribute__((aligned(1024))) float lst[2][64];  // a step's 32 log2-lse and 32 delta
+  const int nb = a.head->nblocks, H = a.k.H * a.parts, id = blockIdx.x;
   if (id >= nb * H) return;
   PaSpan sp = a.blocks[id / H];
   // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
   if (a.causal) sp.row0 = (sp.len - 1) / a.block_rows * a.block_rows - sp.row0;
-  const int hk = id % H, G = a.q.H / H;
+  const int G = a.q.H / a.k.H, per = (G + a.parts - 1) / a.parts;
+  const int part = id % H % a.parts, hk = id % H / a.parts;
+  const int h0 = hk * G + part * per, h1 = min(h0 + per, (hk + 1) * G);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1], &sq = a.stream[2], &sg = a.stream[3];
   const int t0 = a.causal ? sp.row0 >> 5 : 0, t1 = (sp.len + 31) >> 5;
   PaRange own, rq, rg;
-  pa_scan(sk.info, H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
-  pa_scan(sv.info, H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
-  for (int h = hk * G; h < (hk + 1) * G; ++h) {
+  pa_scan(sk.info, a.k.H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
+  pa_scan(sv.info, a.k.H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
+  for (int h = hk * G; h < (hk + 1) * G; ++h) {  // (the parts of one block decide alike)
     pa_scan(sq.info, a.q.H, h, sp.tile0 + (t0 >> 1), sp.tile0 + ((t1 + 1) >> 1), rq);
     pa_scan(sg.info, a.q.H, h, sp.tile0 + (t0 >> 1), sp.tile0 + ((t1 + 1) >> 1), rg);
   }
   rq.slow |= own.slow;
   const bool slow_q = pa_slow(rq), slow_g = pa_slow(rg);
   if (slow_q || slow_g) {
-    pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&ls[0][0]));
+    pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
     return;
   }
+  const PaStage<DP> fq(lq[0]), fg(lg[0]);
   const int r0 = sp.row0 + 32 * w, j = r0 + (lane & 31);
-  const bool busy = r0 < sp.len;
+  const int nt = t1 - t0, steps = nt * (h1 - h0);
+  struct At {  // a step's head and 32 queries
+    int h, t;
+    VH_DEV void next(int t0, int t1) {
+      if (++t == t1) {
+        t = t0;
+        ++h;
+      }
+    }
+  };
+  auto tile = [&](At x) { return (int64_t)(sp.tile0 + (x.t >> 1)) * a.q.H + x.h; };
+  auto stage = [&](At x, int st) {
+    const int64_t at = tile(x) * (2 * SUB) + (x.t & 1) * SUB;
+    pa_copy<NW, 2 * SUB>(sq.n + at, lq[st]);
+    pa_copy<NW, 2 * SUB>(sg.n + at, lg[st]);
+    if (threadIdx.x < 16) pa_copy16(a.stat + tile(x) * 128 + (x.t & 1) * 64 + threadIdx.x * 4, lst[st]);
+  };
+  At now{h0, t0}, ahead{h0, t0};  // ahead: the last step staged
+  if (steps > 0) stage(ahead, 0);
   PaFrag k[KS], v[KS];
   const int ek = pa_own<DP>(a.k, sp, a.D, j, hk, k), ev = pa_own<DP>(a.v, sp, a.D, j, hk, v);
   const float cs = a.scale * PA_LOG2E;
-  const int nt = t1 - t0, steps = nt * G;
-  auto stage = [&](int n, int b) {
-    const int h = hk * G + n / nt, t = t0 + n % nt;
-    const int64_t tile = (int64_t)(sp.tile0 + (t >> 1)) * a.q.H + h, at = tile * (2 * SUB) + (t & 1) * SUB;
-    pa_copy<NW, 2 * SUB>(sq.n + at, ls[b]);
-    pa_copy<NW, 2 * SUB>(sq.tr + at, ls[b] + SUB);
-    pa_copy<NW, 2 * SUB>(sg.n + at, ls[b] + 2 * SUB);
-    pa_copy<NW, 2 * SUB>(sg.tr + at, ls[b] + 3 * SUB);
-    if (threadIdx.x < 16) pa_copy16(a.stat + tile * 128 + (t & 1) * 64 + threadIdx.x * 4, lst[b]);
-  };
   pa_f16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dk[db] = dv[db] = pa_f16{};
-  int eqc = 0, egc = 0, g = 126;
-  float gs = 0x1p126f;
-  stage(0, 0);
+  int egc = 0, g = 126, eqn = 0, egn = 0;
+  const bool busy = r0 < sp.len;
+  if (steps > 0) {
+    eqn = sq.info[tile(now)];
+    egn = sg.info[tile(now)];
+  }
   for (int n = 0; n < steps; ++n) {
-    const int h = hk * G + n / nt, t = t0 + n % nt;
-    const int64_t it = (int64_t)(sp.tile0 + (t >> 1)) * a.q.H + h;
-    const int eq = sq.info[it], eg = sg.info[it];
     pa_arrived();
-    const int b = n & 1;
-    if (n + 1 < steps) stage(n + 1, b ^ 1);
-    if (!busy || (a.causal && 32 * t + 31 < r0)) continue;
+    const int b = n & 1, t = now.t, eq = eqn, eg = egn;
+    now.next(t0, t1);
+    if (n + 1 < steps) {
+      ahead.next(t0, t1);
+      stage(ahead, b ^ 1);
+      eqn = sq.info[tile(now)];
+      egn = sg.info[tile(now)];
+    }
+    if (!busy || (a.causal && 32 * t + 31 < r0)) continue;  // no query of the step sees a key of the wave
+    const float ps = pa_ldexp(1.0f, pa_shift(eg, egc, dv));
     pa_f16 s{}, dp{};
 #pragma unroll
-    for (int c = 0; c < KS; ++c) pa_mma(pa_frag(ls[b], c, KS), k[c], s);
+    for (int c = 0; c < KS; ++c) pa_mma(fq.rows(b, c), k[c], s);
+    if (a.causal && 32 * t < r0 + 31) {  // a query before the lane's key
 #pragma unroll
-    for (int c = 0; c < KS; ++c) pa_mma(pa_frag(ls[b] + 2 * SUB, c, KS), v[c], dp);
-    const float c = pa_ldexp(cs, ek + (eq == PA_ZERO ? 0 : eq) - 2 * PA_E);
+      for (int r = 0; r < 16; ++r)
+        if (32 * t + 8 * (r >> 2) + 4 * hf + (r & 3) < j) s[r] = -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < KS; ++c) pa_mma(fg.rows(b, c), v[c], dp);
+    const float c = fmaxf(pa_ldexp(cs, ek + (eq == PA_ZERO ? 0 : eq) - 2 * PA_E), 0x1p-126f);
     const float cg = pa_ldexp(1.0f, ev + (eg == PA_ZERO ? 0 : eg) - 2 * PA_E);
     // Register r is query 32 t + 8 (r / 4) + 4 hf + r % 4, the lane's column key j.
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const pa_f4 ls4 = *reinterpret_cast<const pa_f4*>(&lst[b][8 * y + 4 * hf]);
-      const pa_f4 dl4 = *reinterpret_cast<const pa_f4*>(&lst[b][32 + 8 * y + 4 * hf]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * y + e;
-        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ls4[e]));
-        dp[r] = fmaf(dp[r], cg, -dl4[e]);
-      }
+      for (int e = 0; e < 4; ++e) s[4 * y + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + e], c, -ls4[e]));
     }
-    if (a.causal && 32 * t < r0 + 31) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (32 * t + 8 * (r >> 2) + 4 * hf + (r & 3) < j) s[r] = 0.0f;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-    pa_units_to(eq, eqc, dk);
-    pa_units_to(eg, egc, dv);
-    pa_fit(dp, gs, g, dk);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const PaFrag fp = pa_split8([&](int x) { return s[8 * u + x]; });
+      const PaFrag f = pa_split8([&](int y) { return s[8 * u + y] * ps; });
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(pa_frag(ls[b] + 3 * SUB, 2 * db + u, 2 * DB), fp, dv[db]);
-      const PaFrag fs = pa_split8([&](int x) { return dp[8 * u + x] * gs; });
+      for (int db = 0; db < DB; ++db) pa_mma(fg.cols(b, db, u), f, dv[db]);
+    }
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(pa_frag(ls[b] + SUB, 2 * db + u, 2 * DB), fs, dk[db]);
+    for (int y = 0; y < 4; ++y) {
+      const pa_f4 dl4 = *reinterpret_cast<const pa_f4*>(&lst[b][32 + 8 * y + 4 * hf]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * y + e] *= fmaf(dp[4 * y + e], cg, -dl4[e]);
+    }
+    const float gs = pa_fit(s, eq == PA_ZERO ? 0 : eq - rq.hi, g, dk);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const PaFrag f = pa_split8([&](int y) { return s[8 * u + y] * gs; });
+#pragma unroll
+      for (int db = 0; db < DB; ++db) pa_mma(fq.cols(b, db, u), f, dk[db]);
     }
   }
   if (j >= sp.len) return;
   const int64_t tok = (int64_t)sp.start + j;
-  pa_store<DB>(a.dk + tok * a.dk_t + hk * a.dk_h, a.dk_vec, a.D, dk,
-               [&](float x) { return pa_ldexp(x * a.scale, eqc - 2 * PA_E - g); });
-  pa_store<DB>(a.dv + tok * a.dv_t + hk * a.dv_h, a.dv_vec, a.D, dv,
-               [&](float x) { return pa_ldexp(x, egc - 2 * PA_E); });
+  const bool whole = a.parts == 1;
+  float* ok = whole ? a.dk + tok * a.dk_t + hk * a.dk_h : a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * DP;
+  float* ov = whole ? a.dv + tok * a.dv_t + hk * a.dv_h : a.join + ((((int64_t)part * 2 + 1) * a.T + tok) * a.k.H + hk) * DP;
+  pa_store<DB>(ok, whole ? a.dk_vec : 1, whole ? a.D : DP, dk, [&](float y) { return pa_ldexp(y * a.scale, rq.hi - PA_E - PA_PV - g); });
+  pa_store<DB>(ov, whole ? a.dv_vec : 1, whole ? a.D : DP, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
+}
+
+// dk and dv of each token in a sequence: the parts' sums, in order. Grid: (tiles,
+// key heads, dk and dv).
+template <int DP>
+VH_DEV void pa_join_impl(const PaArgs& a) {
+  if ((int)blockIdx.x >= a.head->ntiles) return;
+  const PaSpan sp = a.tiles[blockIdx.x];
+  const int hk = blockIdx.y, z = blockIdx.z, rows = min(64, sp.len - sp.row0);
+  float* out = z ? a.dv : a.dk;
+  const int64_t ot = z ? a.dv_t : a.dk_t, oh = z ? a.dv_h : a.dk_h, step = (int64_t)2 * a.T * a.k.H * DP;
+  for (int u = threadIdx.x; u < rows * (DP / 4); u += 256) {
+    const int64_t tok = (int64_t)sp.start + sp.row0 + u / (DP / 4);
+    const int d = u % (DP / 4) * 4;
+    const float* p = a.join + (((int64_t)z * a.T + tok) * a.k.H + hk) * DP + d;
+    pa_f4 s = *reinterpret_cast<const pa_f4*>(p);
+    for (int k = 1; k < a.parts; ++k) s += *reinterpret_cast<const pa_f4*>(p + k * step);
+    float* q = out + tok * ot + hk * oh + d;
+    if (z ? a.dv_vec : a.dk_vec) {
+      if (d < a.D) *reinterpret_cast<pa_f4*>(q) = s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < a.D) q[e] = s[e];
+    }
+  }
 }

@@ -123,10 +123,19 @@ constexpr int64_t kPaMatrixD = 128;
 int pa_padded(int64_t D) { return (int)(cdiv(D, 32) * 32); }
 int pa_block_rows(int64_t D) { return D <= kPaMatrixD ? 128 : 64; }
 
-// The workspace, in the order its parts are laid out. Streams: k, v, q, dout; each in
-// fragments by rows (n) and by columns (t) as far as the kernels read them.
+// Workgroups that share a key head's query heads in dk and dv: as many as bring the blocks
+// to kPaJoinBlocks, where a block's first keys meet every query after them. [8192] tokens, 16
+// query heads on 2 of 128: 128 workgroups take 7.2 ms for what 1024 do in PLACEHOLDER.
+constexpr int64_t kPaJoinBlocks = 1024;
+int pa_parts(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
+  if (D > kPaMatrixD) return 1;
+  const int64_t G = Hq / Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk)));
+  return (int)cdiv(G, per);
+}
+
+// The workspace, in the order its parts are laid out. Streams: k, v, q, dout.
 struct PaScratch {
-  size_t head, tiles, blocks, delta, stat, n[4], t[4], info[4], total;
+  size_t head, tiles, blocks, delta, stat, join, n[4], info[4], total;
   PaScratch(int64_t T, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, bool backward) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -141,12 +150,12 @@ struct PaScratch {
     delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
     const bool mm = D <= kPaMatrixD;
     stat = take(mm && backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
+    const int parts = pa_parts(T, Hq, Hk, D);
+    join = take(backward && parts > 1 ? sizeof(float) * 2 * (size_t)(parts * T * Hk * pa_padded(D)) : 0);
     for (int i = 0; i < 4; ++i) {
-      const bool used = mm && (backward || i < 2);
-      const size_t tiles_h = units * (size_t)(i < 2 ? Hk : Hq), bytes = tiles_h * 256 * (size_t)pa_padded(D);
-      n[i] = take(used && (backward || i == 0) ? bytes : 0);
-      t[i] = take(used && (backward ? i != 1 : i == 1) ? bytes : 0);
-      info[i] = take(used ? sizeof(int32_t) * tiles_h : 0);
+      const size_t tiles_h = mm && (backward || i < 2) ? units * (size_t)(i < 2 ? Hk : Hq) : 0;
+      n[i] = take(tiles_h * 256 * (size_t)pa_padded(D));
+      info[i] = take(tiles_h * sizeof(int32_t));
     }
     total = at;
   }
@@ -208,6 +217,8 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
   a.blocks = reinterpret_cast<PaSpan*>(p + l.blocks);
   a.delta = reinterpret_cast<float*>(p + l.delta);
   a.stat = reinterpret_cast<float*>(p + l.stat);
+  a.join = reinterpret_cast<float*>(p + l.join);
+  a.parts = backward ? pa_parts(c->q.T, c->q.H, c->k.H, c->q.D) : 1;
   a.grad = -1;
   if (c->q.D > kPaMatrixD) {
     VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
@@ -216,10 +227,8 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
   const PaTensor t[4] = {a.k, a.v, a.q, a.g};
   const int streams = backward ? 4 : 2;
   for (int i = 0; i < streams; ++i) {
-    const bool by_rows = backward || i == 0, by_cols = backward ? i != 1 : i == 1;
-    a.stream[i] = PaStream{t[i], by_rows ? reinterpret_cast<uint16_t*>(p + l.n[i]) : nullptr,
-                           by_cols ? reinterpret_cast<uint16_t*>(p + l.t[i]) : nullptr,
-                           reinterpret_cast<int32_t*>(p + l.info[i]), i < 2 ? VH_PA_SPAN_KV : VH_PA_SPAN_Q};
+    a.stream[i] = PaStream{t[i], reinterpret_cast<uint16_t*>(p + l.n[i]), reinterpret_cast<int32_t*>(p + l.info[i]),
+                           i < 2 ? VH_PA_SPAN_KV : VH_PA_SPAN_Q};
   }
   if (backward) a.grad = 3;
   return launch("vh_pa_prep_" + std::to_string(pa_padded(c->q.D)), a.max_tiles, backward ? c->q.H : c->k.H, streams, 256,
@@ -455,7 +464,8 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
     return launch("vh_pa_rows_dkdv", a.max_blocks, c.k.H, 1, 256, s, a);
   }
   const std::string dp = std::to_string(pa_padded(c.q.D));
-  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H, 1, 1, 256, s, a));
+  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H * a.parts, 1, 1, 256, s, a));
+  if (a.parts > 1) VH_TRY(launch("vh_pa_join_" + dp, a.max_tiles, c.k.H, 2, 256, s, a));
   return launch("vh_pa_dq_" + dp, a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }
 

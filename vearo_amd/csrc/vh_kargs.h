@@ -471,8 +471,7 @@ struct PaTensor {
 };
 struct PaStream {  // a tensor that the matrix kernels stream, split by the prepare launch
   PaTensor t;
-  uint16_t* n;      // fragments by rows and by columns, or null
-  uint16_t* tr;
+  uint16_t* n;      // [tiles][H] fragments
   int32_t* info;    // [tiles][H] exponents
   int32_t span;     // rows of a tile may differ by so many powers of two
 };
@@ -481,7 +480,9 @@ struct PaArgs {
   PaStream stream[4];      // k, v, q, g (forward: the first two)
   int32_t grad;            // the gradient's stream (the prepare launch forms delta with it), or -1
   int32_t out_vec, dq_vec, dk_vec, dv_vec;  // rows may be written as 16-byte units
-  float* stat;             // [tiles][Hq][2][32 log2-lse - 14, 32 delta]
+  int32_t parts;           // workgroups that divide a key head's query heads (dk and dv)
+  float* join;             // parts > 1: [parts][dk, dv][T][Hk][D padded] sums
+  float* stat;             // [tiles][Hq][2][32 log2-lse - 11, 32 delta]
   float* out;              // forward
   int64_t out_t, out_h;
   float* lse;              // [Hq][T]
