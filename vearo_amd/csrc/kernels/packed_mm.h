@@ -342,32 +342,34 @@ VH_DEV int pa_shift(int e, int& cur, pa_f16 (&acc)[DB]) {
   return 0;
 }
 
-// Looks over the exponents of tiles t0 .. t1 - 1 of a stream: whether one is not for the
-// matrix kernels or, over all calls with the same lo, hi, they differ too much.
+// The exponents of a stream's tiles that a workgroup looked over: whether one is not for
+// the matrix kernels, or they differ too much.
 struct PaRange {
-  int lo = 10000, hi = -10000;
+  float lo = 1e4f, hi = -1e4f;
   bool slow = false;
-};
-VH_DEV void pa_scan(const int32_t* info, int64_t H, int h, int t0, int t1, PaRange& r) {
-  for (int t = t0 + (threadIdx.x & 63); t < t1; t += 64) {
-    const int e = info[t * H + h];
-    if (e == PA_SLOW) r.slow = true;
-    else if (e != PA_ZERO) {
-      r.lo = min(r.lo, e);
-      r.hi = max(r.hi, e);
+  VH_DEV void add(int e) {
+    slow |= e == PA_SLOW;
+    if (e < PA_ZERO) {
+      lo = fminf(lo, (float)e);
+      hi = fmaxf(hi, (float)e);
     }
   }
-}
-VH_DEV bool pa_slow(PaRange& r) {
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    r.lo = min(r.lo, __shfl_xor(r.lo, k, 64));
-    r.hi = max(r.hi, __shfl_xor(r.hi, k, 64));
+  // Over the wave's lanes; the largest in `top` (0 if all are zeros).
+  VH_DEV bool any_slow(int& top) {
+    hi = group_max<64>(hi);
+    lo = -group_max<64>(-lo);
+    top = hi < -1e3f ? 0 : __builtin_amdgcn_readfirstlane((int)hi);
+    return __builtin_amdgcn_ballot_w64(slow) != 0 || hi - lo > (float)PA_SPAN_TILES;
   }
-  r.hi = __builtin_amdgcn_readfirstlane(r.hi);
-  const bool slow = __builtin_amdgcn_ballot_w64(r.slow) != 0 || r.hi - r.lo > PA_SPAN_TILES;
-  if (r.hi < -1000) r.hi = 0;  // (zeros only)
-  return slow;
+};
+// Tiles t0 .. t1 - 1 of head h of two streams with H heads.
+VH_DEV void pa_scan(const PaStream& x, const PaStream& y, int H, int h, int t0, int t1, PaRange& rx, PaRange& ry) {
+  for (int t = t0 + (threadIdx.x & 63); t < t1; t += 64) {
+    const int64_t at = (int64_t)t * H + h;
+    const int ex = x.info[at], ey = y.info[at];
+    rx.add(ex);
+    ry.add(ey);
+  }
 }
 
 // -------------------------------------------------------------------- forward --
@@ -384,21 +386,13 @@ template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
   __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
-  const int nb = a.head->nblocks, H = a.q.H, id = blockIdx.x;
-  if (id >= nb * H) return;
-  const PaSpan sp = a.blocks[id / H];
+  const int H = a.q.H, id = blockIdx.x;
+  const PaSpan sp = a.blocks[id / H];  // (inside the table, also where it is not written)
+  if (id >= a.head->nblocks * H) return;
   const int h = id % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
-  PaRange rk, rv;
-  pa_scan(sk.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk);
-  pa_scan(sv.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rv);
-  rv.slow |= rk.slow;
-  if (pa_slow(rv)) {
-    pa_rows<0>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
-    return;
-  }
   const PaStage<DP> fk(lk[0]), fv(lv[0]);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
   const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
@@ -410,6 +404,15 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   if (nt > 1) stage(sk.n, 1, lk[1]);
   PaFrag q[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q);
+  PaRange rk, rv;
+  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk, rv);
+  rv.slow |= rk.slow;
+  int top;
+  if (rv.any_slow(top)) {
+    pa_arrived();  // (nothing on its way into the rows' LDS)
+    pa_rows<0>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
+    return;
+  }
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
   const float cs = a.scale * PA_LOG2E;
   pa_f16 o[DB], s{};
@@ -523,21 +526,13 @@ template <int DP, int NW>
 VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
   __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
-  const int nb = a.head->nblocks, H = a.q.H, id = blockIdx.x;
-  if (id >= nb * H) return;
+  const int H = a.q.H, id = blockIdx.x;
   const PaSpan sp = a.blocks[id / H];
+  if (id >= a.head->nblocks * H) return;
   const int h = id % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
-  PaRange rk, rv;
-  pa_scan(sk.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk);
-  pa_scan(sv.info, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rv);
-  rk.slow |= rv.slow;
-  if (pa_slow(rk)) {
-    pa_rows<1>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
-    return;
-  }
   const PaStage<DP> fk(lk[0]), fv(lv[0]);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
   const bool live = i < sp.len;
@@ -549,6 +544,15 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   stage(sv.n, 0, lv[0]);
   PaFrag q[KS], gq[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q), eg = pa_own<DP>(a.g, sp, a.D, i, h, gq);
+  PaRange rk, rv;
+  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk, rv);
+  rk.slow |= rv.slow;
+  int top;
+  if (rk.any_slow(top)) {
+    pa_arrived();
+    pa_rows<1>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
+    return;
+  }
   const int64_t tok = (int64_t)sp.start + i;
   const float lse = live ? a.lse[(int64_t)h * a.T + tok] * PA_LOG2E : 0.0f;
   const float dl = live ? a.delta[(int64_t)h * a.T + tok] : 0.0f;
@@ -588,7 +592,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] *= fmaf(dp[r], cg, -dl);
-    const float gs = pa_fit(s, ek == PA_ZERO ? 0 : ek - rk.hi, g, acc);
+    const float gs = pa_fit(s, ek == PA_ZERO ? 0 : ek - top, g, acc);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const PaFrag f = pa_split8([&](int k) { return s[8 * u + k] * gs; });
@@ -598,7 +602,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   }
   if (!live) return;
   pa_store<DB>(a.dq + tok * a.dq_t + h * a.dq_h, a.dq_vec, a.D, acc,
-               [&](float v) { return pa_ldexp(v * a.scale, rk.hi - PA_E - g); });
+               [&](float v) { return pa_ldexp(v * a.scale, top - PA_E - g); });
 }
 
 // dk and dv: a workgroup per block of 32 NW keys, key head and part of its query heads,
@@ -612,9 +616,9 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
   __shared__ __attribute__((aligned(1024))) uint16_t lq[2][SUB], lg[2][SUB];
   __shared__ __attribute__((aligned(1024))) float lst[2][64];  // a step's 32 log2-lse and 32 delta
-  const int nb = a.head->nblocks, H = a.k.H * a.parts, id = blockIdx.x;
-  if (id >= nb * H) return;
+  const int H = a.k.H * a.parts, id = blockIdx.x;
   PaSpan sp = a.blocks[id / H];
+  if (id >= a.head->nblocks * H) return;
   // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
   if (a.causal) sp.row0 = (sp.len - 1) / a.block_rows * a.block_rows - sp.row0;
   const int G = a.q.H / a.k.H, per = (G + a.parts - 1) / a.parts;
@@ -623,19 +627,6 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1], &sq = a.stream[2], &sg = a.stream[3];
   const int t0 = a.causal ? sp.row0 >> 5 : 0, t1 = (sp.len + 31) >> 5;
-  PaRange own, rq, rg;
-  pa_scan(sk.info, a.k.H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
-  pa_scan(sv.info, a.k.H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), own);
-  for (int h = hk * G; h < (hk + 1) * G; ++h) {  // (the parts of one block decide alike)
-    pa_scan(sq.info, a.q.H, h, sp.tile0 + (t0 >> 1), sp.tile0 + ((t1 + 1) >> 1), rq);
-    pa_scan(sg.info, a.q.H, h, sp.tile0 + (t0 >> 1), sp.tile0 + ((t1 + 1) >> 1), rg);
-  }
-  rq.slow |= own.slow;
-  const bool slow_q = pa_slow(rq), slow_g = pa_slow(rg);
-  if (slow_q || slow_g) {
-    pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
-    return;
-  }
   const PaStage<DP> fq(lq[0]), fg(lg[0]);
   const int r0 = sp.row0 + 32 * w, j = r0 + (lane & 31);
   const int nt = t1 - t0, steps = nt * (h1 - h0);
@@ -659,6 +650,18 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   if (steps > 0) stage(ahead, 0);
   PaFrag k[KS], v[KS];
   const int ek = pa_own<DP>(a.k, sp, a.D, j, hk, k), ev = pa_own<DP>(a.v, sp, a.D, j, hk, v);
+  PaRange ok, ov, rq, rg;
+  pa_scan(sk, sv, a.k.H, hk, sp.tile0 + (sp.row0 >> 6), sp.tile0 + ((min(sp.len, sp.row0 + 32 * NW) + 63) >> 6), ok, ov);
+  for (int h = hk * G; h < (hk + 1) * G; ++h)  // (the parts of one block decide alike)
+    pa_scan(sq, sg, a.q.H, h, sp.tile0 + (t0 >> 1), sp.tile0 + ((t1 + 1) >> 1), rq, rg);
+  rq.slow |= ok.slow | ov.slow;
+  int topq, topg;
+  const bool slow_q = rq.any_slow(topq), slow_g = rg.any_slow(topg);
+  if (slow_q || slow_g) {
+    pa_arrived();
+    pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
+    return;
+  }
   const float cs = a.scale * PA_LOG2E;
   pa_f16 dk[DB], dv[DB];
 #pragma unroll
@@ -712,7 +715,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * y + e] *= fmaf(dp[4 * y + e], cg, -dl4[e]);
     }
-    const float gs = pa_fit(s, eq == PA_ZERO ? 0 : eq - rq.hi, g, dk);
+    const float gs = pa_fit(s, eq == PA_ZERO ? 0 : eq - topq, g, dk);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const PaFrag f = pa_split8([&](int y) { return s[8 * u + y] * gs; });
@@ -723,10 +726,10 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   if (j >= sp.len) return;
   const int64_t tok = (int64_t)sp.start + j;
   const bool whole = a.parts == 1;
-  float* ok = whole ? a.dk + tok * a.dk_t + hk * a.dk_h : a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * DP;
-  float* ov = whole ? a.dv + tok * a.dv_t + hk * a.dv_h : a.join + ((((int64_t)part * 2 + 1) * a.T + tok) * a.k.H + hk) * DP;
-  pa_store<DB>(ok, whole ? a.dk_vec : 1, whole ? a.D : DP, dk, [&](float y) { return pa_ldexp(y * a.scale, rq.hi - PA_E - PA_PV - g); });
-  pa_store<DB>(ov, whole ? a.dv_vec : 1, whole ? a.D : DP, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
+  float* const to_k = whole ? a.dk + tok * a.dk_t + hk * a.dk_h : a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * DP;
+  float* const to_v = whole ? a.dv + tok * a.dv_t + hk * a.dv_h : a.join + ((((int64_t)part * 2 + 1) * a.T + tok) * a.k.H + hk) * DP;
+  pa_store<DB>(to_k, whole ? a.dk_vec : 1, whole ? a.D : DP, dk, [&](float y) { return pa_ldexp(y * a.scale, topq - PA_E - PA_PV - g); });
+  pa_store<DB>(to_v, whole ? a.dv_vec : 1, whole ? a.D : DP, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
 }
 
 // dk and dv of each token in a sequence: the parts' sums, in order. Grid: (tiles,
