@@ -235,6 +235,11 @@ VH_DEV void pa_arrived() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
 }
+// A tile's exponent, the same for all lanes, by the scalar unit: a vector load would wait
+// for the copies in flight before it. (Constant memory here: the prepare launch wrote it.)
+typedef const __attribute__((address_space(4))) int32_t* PaInfo;
+VH_DEV PaInfo pa_info(const int32_t* p) { return (PaInfo)(uintptr_t)p; }
+
 // What a wave reads of a 32-token stage, 64 DP halves: [part][16 elements][piece].
 template <int DP>
 struct PaStage {
@@ -377,11 +382,8 @@ VH_DEV void pa_scan(const PaStream& x, const PaStream& y, int H, int h, int t0, 
 // 32 through two LDS stages. A step multiplies the next step's S while its own P is formed
 // and multiplied by V: the matrix unit and the vector unit (exp is a quarter rate) have
 // about as much to do, and a wave alone would have them take turns. So K runs one step
-// ahead of V. The running maximum m of a row (in log2 units, scaled) is raised only when
-// a step's maximum passes it by more than PA_LAG, so that most steps leave the
-// accumulators alone; P is held at 2^PA_PSHIFT times its value against that m, below 2^14.
-#define PA_LAG 8.0f
-#define PA_PSHIFT 3.0f
+// ahead of V. The accumulators are multiplied over at every step, to the new maximum and to
+// V's units at once: a branch around it costs the usual path more in copied registers.
 template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
@@ -420,45 +422,48 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   for (int db = 0; db < DB; ++db) o[db] = pa_f16{};
   float m = -INFINITY, l = 0.0f;
   int ev = 0;
-  // Steps that some row of the wave sees.
+  // Steps that some row of the wave sees: all but the last are seen whole.
   const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
   // The steps' exponents, read one step ahead.
-  const int32_t *ik = sk.info + (int64_t)sp.tile0 * a.k.H + hk, *iv = sv.info + (int64_t)sp.tile0 * a.k.H + hk;
+  const PaInfo ik = pa_info(sk.info) + ((int64_t)sp.tile0 * a.k.H + hk), iv = pa_info(sv.info) + ((int64_t)sp.tile0 * a.k.H + hk);
   int ekn = *ik, evn = *iv;
-  auto step = [&](int t, int ek, int evt, auto more) {
-    const int b = t & 1;
+  // Step t's V and step t + 1's K are in LDS; V of t + 1 and K of t + 2 go out.
+  auto arrive = [&](int t) {
+    if (t) pa_arrived();
+    if (t + 1 < nt) stage(sv.n, t + 1, lv[(t + 1) & 1]);
+    if (t + 2 < nt) stage(sk.n, t + 2, lk[t & 1]);
+  };
+  auto step = [&](int t, auto last) {
+    const int b = t & 1, ek = ekn, evt = evn;
+    const int64_t ahead = (int64_t)(min(t + 1, nt - 1) >> 1) * a.k.H;
+    ekn = ik[ahead];
+    evn = iv[ahead];
     const float c = fmaxf(pa_ldexp(cs, eq + (ek == PA_ZERO ? 0 : ek) - 2 * PA_E), 0x1p-126f);
-    if (32 * t + 32 > (a.causal ? r0 + 1 : sp.len)) {  // some row does not see all of it
+    pa_f16 next{};
+    if constexpr (decltype(last)::value) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (32 * t + 4 * hf + 8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+    } else {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) pa_mma(fk.rows(b ^ 1, k), q[k], next);
     }
     float mt = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-    mt = pa_max_halves(mt) * c;
-    if (__builtin_amdgcn_ballot_w64(mt > m + PA_LAG) != 0) {
-      const float mn = fmaxf(m, mt), al = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= al;
+    const float mn = fmaxf(m, pa_max_halves(mt) * c), al = __builtin_amdgcn_exp2f(m - mn), ms = mn - (float)PA_E;
+    const float f = pa_ldexp(al, evt == PA_ZERO ? 0 : ev - evt);
+    m = mn;
+    ev = evt == PA_ZERO ? ev : evt;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] *= al;
-    }
-    const int sh = pa_shift(evt, ev, o);
-    const float ms = m - PA_PSHIFT - (float)sh;
-    pa_f16 next{};
-    if constexpr (decltype(more)::value) {
-#pragma unroll
-      for (int k = 0; k < KS; ++k) pa_mma(fk.rows(b ^ 1, k), q[k], next);
-    }
+      for (int r = 0; r < 16; ++r) o[db][r] *= f;
+    l *= al;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ms));
-    float ls = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ls += s[r];
-    l = fmaf(ls, pa_ldexp(1.0f, -sh), l);
+    for (int r = 0; r < 16; ++r) l += s[r];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const PaFrag p = pa_split8([&](int k) { return s[8 * g + k]; });
@@ -467,24 +472,22 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
     }
     s = next;
   };
-  // Arrived: V of step t and K of step t + 1; then V of t + 1 and K of t + 2 go out.
   pa_arrived();
   if (mine > 0) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) pa_mma(fk.rows(0, k), q[k], s);
   }
-  for (int t = 0; t < nt; ++t) {
-    if (t) pa_arrived();
-    else __syncthreads();  // (K of step 0 has been read)
-    if (t + 1 < nt) stage(sv.n, t + 1, lv[(t + 1) & 1]);
-    if (t + 2 < nt) stage(sk.n, t + 2, lk[t & 1]);
-    const int ek = ekn, evt = evn;
-    const int64_t ahead = (int64_t)(min(t + 1, nt - 1) >> 1) * a.k.H;
-    ekn = ik[ahead];
-    evn = iv[ahead];
-    if (t + 1 < mine) step(t, ek, evt, std::true_type{});
-    else if (t < mine) step(t, ek, evt, std::false_type{});
+  __syncthreads();  // (K of step 0 has been read)
+  int t = 0;
+  for (; t + 1 < mine; ++t) {
+    arrive(t);
+    step(t, std::false_type{});
   }
+  if (t < mine) {
+    arrive(t);
+    step(t++, std::true_type{});
+  }
+  for (; t < nt; ++t) arrive(t);
   if (r0 >= sp.len) return;
   l = pa_sum_halves(l);
   if (i >= sp.len) return;
@@ -492,7 +495,7 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   const float inv = 1.0f / l;
   pa_store<DB>(a.out + tok * a.out_t + h * a.out_h, a.out_vec, a.D, o,
                [&](float v) { return pa_ldexp(v * inv, ev - PA_E); });
-  if (hf == 0) a.lse[(int64_t)h * a.T + tok] = (m - PA_PSHIFT) * PA_LN2 + logf(l);
+  if (hf == 0) a.lse[(int64_t)h * a.T + tok] = (m - (float)PA_E) * PA_LN2 + logf(l);
 }
 
 // -------------------------------------------------------------------- backward --
@@ -563,7 +566,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
   for (int db = 0; db < DB; ++db) acc[db] = pa_f16{};
   int g = 126;
   const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
-  const int32_t *ik = sk.info + (int64_t)sp.tile0 * a.k.H + hk, *iv = sv.info + (int64_t)sp.tile0 * a.k.H + hk;
+  const PaInfo ik = pa_info(sk.info) + ((int64_t)sp.tile0 * a.k.H + hk), iv = pa_info(sv.info) + ((int64_t)sp.tile0 * a.k.H + hk);
   int ekn = *ik, evn = *iv;
   for (int t = 0; t < nt; ++t) {
     pa_arrived();
@@ -669,8 +672,8 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   int egc = 0, g = 126, eqn = 0, egn = 0;
   const bool busy = r0 < sp.len;
   if (steps > 0) {
-    eqn = sq.info[tile(now)];
-    egn = sg.info[tile(now)];
+    eqn = pa_info(sq.info)[tile(now)];
+    egn = pa_info(sg.info)[tile(now)];
   }
   for (int n = 0; n < steps; ++n) {
     pa_arrived();
@@ -679,8 +682,8 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
     if (n + 1 < steps) {
       ahead.next(t0, t1);
       stage(ahead, b ^ 1);
-      eqn = sq.info[tile(now)];
-      egn = sg.info[tile(now)];
+      eqn = pa_info(sq.info)[tile(now)];
+      egn = pa_info(sg.info)[tile(now)];
     }
     if (!busy || (a.causal && 32 * t + 31 < r0)) continue;  // no query of the step sees a key of the wave
     const float ps = pa_ldexp(1.0f, pa_shift(eg, egc, dv));
