@@ -486,12 +486,14 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
 size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D, int backward);
 
 /* loss[0] = mean over the counted rows r of -log_softmax(x[r] w^T)[targets[r]], without
- * keeping the [R, V] logits: they are formed in pieces of rows, in scratch. x: R rows of D,
+ * keeping the [R, V] logits: a forward alone reduces them as they are formed, a gradient
+ * forms them in pieces of rows, in scratch (at most 1 GiB of logits, 256 rows at least).
+ * An infinity in x or w counts as NaN. x: R rows of D,
  * ldx floats apart; w: V rows of D, ldw apart; targets: [R] f32 class ids as above, a row
  * whose target equals `ignore` not counted (NaN: none is). No counted row: loss 0.
  * row_stats: [R, 2], each row's max logit and sum of exp(logit - max), kept for the
  * backward (8-byte aligned). scratch: NULL or
- * vh_linear_cross_entropy_scratch_bytes(R, V) bytes. Not under graph capture
+ * vh_linear_cross_entropy_scratch_bytes(R, D, V, 0) bytes (1 with a gradient). Not under graph capture
  * (VH_ERR_UNSUPPORTED: the products inside take workspaces of their own). */
 int vh_linear_cross_entropy_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
                                 float ignore, float* loss, float* row_stats, int64_t R, int64_t D, int64_t V,
@@ -508,7 +510,7 @@ int vh_linear_cross_entropy_fwd_bwd(const float* x, int64_t ldx, const float* w,
                                     float ignore, const float* grad_out, float* loss, float* dx, int64_t lddx,
                                     float* dw, int64_t lddw, int64_t R, int64_t D, int64_t V, void* scratch,
                                     size_t scratch_bytes, void* stream);
-size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t V);
+size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t D, int64_t V, int backward);
 
 /* AdamW update of one parameter tensor in place, moments m and v in device
  * memory, step count t >= 1. Replaces Tensor::adamw_step (tensor.rs:931-1023,

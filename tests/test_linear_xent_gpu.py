@@ -72,7 +72,8 @@ class Xent:
 
 
 @pytest.mark.parametrize("Rr,D,V", [(1, 1, 1), (1, 4, 2), (3, 5, 7), (2, 64, 1), (64, 32, 100), (100, 96, 513), (257, 128, 1000),
-                                    (300, 129, 2049), (1000, 64, 4099), (33, 768, 5003), (17, 16, 70001)])
+                                    (300, 129, 2049), (1000, 64, 4099), (33, 768, 5003), (17, 16, 70001),
+                                    (700, 768, 1000), (129, 1030, 3001), (1500, 250, 1281), (4100, 40, 2050)])
 @pytest.mark.parametrize("ignored", [0.0, 0.4])
 def test_sizes(vh, Rr, D, V, ignored):
     Xent(vh, Rr, D, V, ignored, go=0.75, seed=Rr).check()
@@ -84,10 +85,10 @@ def test_strided_rows(vh, pad, offset):
 
 
 def test_several_pieces(vh):
-    """More rows than a piece holds: 256 rows a piece at this vocabulary."""
-    V = 200003
-    assert vh.lib.vh_linear_cross_entropy_scratch_bytes(600, V) < 4 * 600 * V
-    Xent(vh, 600, 8, V, 0.3).check()
+    """More rows than a piece holds: 512 rows a piece at this vocabulary."""
+    V = 400003
+    assert vh.lib.vh_linear_cross_entropy_scratch_bytes(700, 8, V, 1) < 4 * 700 * V
+    Xent(vh, 700, 8, V, 0.3).check()
 
 
 @pytest.mark.parametrize("ignore", [-100.0, 3.0, math.nan])
@@ -98,23 +99,35 @@ def test_ignored(vh, ignore):
     Xent(vh, 10, 12, 9, ignore=ignore, t=t).check()
 
 
-def test_no_row_counted(vh):
-    c = Xent(vh, 20, 8, 30, t=[-100.0] * 20)
+@pytest.mark.parametrize("sizes", [(20, 8, 30), (400, 512, 2000)])
+def test_no_row_counted(vh, sizes):
+    c = Xent(vh, *sizes, t=[-100.0] * sizes[0])
     c.check()
     got = c.results()
     assert got["loss"][0] == 0 and not got["dx"].any() and not got["dw"].any()
 
 
 @pytest.mark.parametrize("scale", [1e-6, 30.0])
-def test_flat_and_sharp(vh, scale):
-    Xent(vh, 120, 64, 900, scale=scale).check()
+@pytest.mark.parametrize("sizes", [(120, 64, 900), (400, 512, 2000)])
+def test_flat_and_sharp(vh, scale, sizes):
+    Xent(vh, *sizes, scale=scale).check()
+
+
+def test_rows_of_very_different_size(vh):
+    c = Xent(vh, 500, 600, 1500, 0.1, scale=0.05)
+    r = np.random.default_rng(4)
+    c.x *= (10.0 ** r.uniform(-12, 0, (500, 1))).astype(np.float32)
+    c.w *= (10.0 ** r.uniform(-12, 0, (1500, 1))).astype(np.float32)
+    c.x[7] = c.w[9] = 0
+    c.put()
+    c.check()
 
 
 @pytest.mark.parametrize("value,text", [(-1.0, "Target class cannot be negative: -1"),
                                         (50.0, "Target class 50 out of vocab bounds 50")])
 def test_bad_targets(vh, value, text):
-    for which in ("fwd", "fwd_bwd"):
-        c = Xent(vh, 40, 8, 50)
+    for which, sizes in (("fwd", (40, 8, 50)), ("fwd_bwd", (40, 8, 50)), ("fwd", (2000, 3000, 50)), ("fwd_bwd", (2000, 3000, 50))):
+        c = Xent(vh, *sizes)
         c.t[[11, 30]] = value
         c.put()
         c.call(which)
@@ -123,8 +136,9 @@ def test_bad_targets(vh, value, text):
     vh.sync()
 
 
-def test_bad_values_stay_in_their_row(vh):
-    c = Xent(vh, 40, 16, 200)
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+def test_bad_values_stay_in_their_row(vh, sizes):
+    c = Xent(vh, *sizes)
     c.call("fwd")
     c.call("bwd")
     clean = c.results()
@@ -133,7 +147,7 @@ def test_bad_values_stay_in_their_row(vh):
     c.call("fwd")
     c.call("bwd")
     got = c.results()
-    keep = np.arange(40) != 7
+    keep = np.arange(sizes[0]) != 7
     assert np.isnan(got["loss"][0]) and np.isnan(got["dx"][7]).all() and np.isnan(got["dw"]).all()
     np.testing.assert_array_equal(got["dx"][keep], clean["dx"][keep])
     np.testing.assert_array_equal(got["stats"][keep], clean["stats"][keep])
@@ -159,14 +173,14 @@ def test_same_bits_and_streams(vh):
         st.close()
     with pytest.raises(vh.VhError, match="too small"):
         c.call("fwd", vh.DeviceBuffer(64))
-    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(700, 3001))
+    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(700, 64, 3001, 1))
     c.call("fwd_bwd", scratch)
     np.testing.assert_array_equal(c.results()["dw"], want["dw"])
 
 
 def test_no_capture(vh):
     c = Xent(vh, 10, 8, 20)
-    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(10, 20))
+    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(10, 8, 20, 1))
 
     def body(s):
         for which in ("fwd", "bwd", "fwd_bwd"):

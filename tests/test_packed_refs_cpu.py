@@ -216,6 +216,8 @@ def test_scratch_sizes():
     assert L.vh_packed_attention_scratch_bytes(0, 1, 4, 2, 64, 1) == 0
     assert L.vh_packed_attention_scratch_bytes(16384, 8, 12, 4, 64, 1) >= 4 * 12 * 16384
     assert L.vh_qk_norm_rope_bwd_scratch_bytes(0, 64) == 0 < L.vh_qk_norm_rope_bwd_scratch_bytes(1, 1)
-    # Pieces: far below the logits, and no less than 256 rows of them.
-    assert L.vh_linear_cross_entropy_scratch_bytes(16384, 50257) < 4 * 16384 * 50257 // 8
-    assert L.vh_linear_cross_entropy_scratch_bytes(1024, 4000000) >= 4 * 256 * 4000000
+    # A gradient's pieces: below the logits, and no less than 256 rows of them. A forward: none.
+    assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 1) < 4 * 65536 * 50257 // 8
+    assert L.vh_linear_cross_entropy_scratch_bytes(1024, 8, 4000000, 1) >= 4 * 256 * 4000000
+    assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 0) < 4 * 65536 * 50257 // 16
+    assert L.vh_linear_cross_entropy_scratch_bytes(0, 8, 8, 1) == 0

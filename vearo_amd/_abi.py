@@ -204,7 +204,7 @@ SIGNATURES = {
         [fp, c_int64, fp, c_int64, fp, c_float, fp, fp, fp, c_int64, fp, c_int64, c_int64, c_int64, c_int64, c_void_p,
          c_size_t, c_void_p],
     ),
-    "vh_linear_cross_entropy_scratch_bytes": (c_size_t, [c_int64, c_int64]),
+    "vh_linear_cross_entropy_scratch_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
     "vh_adamw_step": (
         c_int,
         [fp, fp, fp, fp, c_int64, c_int32, c_float, c_float, c_float, c_float, c_float, c_void_p],

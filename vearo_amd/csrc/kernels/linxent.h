@@ -5,8 +5,17 @@
 //   dz = (exp(z - max) / sum - 1[target]) * go * inv,  inv = 1 / counted rows,
 // a row whose target is `ignore` not counted and its dz zero; no counted row at all
 // gives loss 0 and dz 0. Memory bound on a piece that the last-level cache mostly holds.
+//
+// The logits come from vh_gemm's products or, where they are many, from lx_logits below:
+// each operand row in two f16 parts under a power of two of its own (packed_mm.h says
+// what that keeps of an f32 value; along a row the smallest elements lose bits below 2^-40
+// of the largest, which is below the sum's own rounding), three products for one where
+// the three bf16 parts of split3.h take six. Only the logits: the gradient's rows hold
+// probabilities over any range of magnitudes, which f16's exponent would cut off, so its two
+// products stay on the bf16 parts.
 #pragma once
 #include "common.h"
+#include "packed_mm.h"
 
 #define LX_BLOCK 512
 
@@ -100,4 +109,220 @@ VH_DEV void lx_loss_impl(const LxLossArgs& a) {
   for (int64_t i = threadIdx.x; i < a.R; i += 1024) s += a.row_loss[i];
   s = team_sum<1024>(s, red);
   if (threadIdx.x == 0) a.loss[0] = s * *a.inv;
+}
+
+// ------------------------------------------------------------- logits, f16 parts --
+// Fragments of 32 rows (blockIdx.x), eight threads a row. A row's power of two comes from
+// its finite elements; infinities and NaN come through as NaN.
+VH_DEV void lx_split_impl(const LxSplitArgs& a) {
+  const int row = threadIdx.x >> 3, c = threadIdx.x & 7;
+  const int64_t r = (int64_t)blockIdx.x * 32 + row;
+  const float* p = a.x + r * a.ld;
+  auto load = [&](int d, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    if (r >= a.rows) return;
+    if (a.vec) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 4)
+        if (d + k < a.D) {
+          const pa_f4 q = *reinterpret_cast<const pa_f4*>(p + d + k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[k + e] = q[e];
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (d + k < a.D) v[k] = p[d + k];
+    }
+  };
+  float m = 0.0f;
+  for (int d = 8 * c; d < a.D; d += 64) {
+    float v[8];
+    load(d, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float x = fabsf(v[k]);
+      m = x < INFINITY ? fmaxf(m, x) : m;
+    }
+  }
+  m = group_max<8>(m);
+  const int e = m > 0.0f ? pa_exp(m) : 0;
+  if (c == 0) a.exp[r] = e;
+  for (int d = 8 * c; d < 16 * a.ke; d += 64) {
+    float v[8];
+    load(d, v);
+    const PaFrag f = pa_split8([&](int k) { return pa_ldexp(v[k], PA_E - e); });
+    const int k = d >> 4;
+    pa_u4* to = reinterpret_cast<pa_u4*>(a.frag) + ((int64_t)blockIdx.x * a.ke + k) * 128 + pa_piece((d >> 3 & 1) * 32 + row, k);
+    to[0] = __builtin_bit_cast(pa_u4, f.h);
+    to[64] = __builtin_bit_cast(pa_u4, f.l);
+  }
+}
+
+// z = x w^T on a tile of 256 entries x 128 rows, four waves of 64 entries x 128 rows, two
+// workgroups a CU (one's epilogue under the other's products). Entries are the rows of
+// the matrix instruction and x's rows its columns, so a row's max and sum of exp are
+// formed in a lane. 16 elements a step, three LDS stages, two on their way.
+VH_DEV void lx_logits_impl(const LxLogitArgs& a) {
+  constexpr int FW = VH_LX_TV / 32, FX = VH_LX_TR / 32, STAGE = (FW + FX) * 1024;  // halves
+  __shared__ __attribute__((aligned(1024))) uint16_t ls[3][STAGE];
+  __shared__ float red[4][VH_LX_TR][2];
+  const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5, li = lane & 31;
+  // XCD x (the hardware deals workgroups out in turn) takes an eighth of the tiles, row
+  // tiles fastest within groups of eight, so that its L2 serves both operands.
+  const int tiles = a.tv * a.tr, xcd = blockIdx.x & 7, lo = (int)((int64_t)tiles * xcd / 8);
+  const int u = lo + (int)(blockIdx.x >> 3);
+  if (u >= (int)((int64_t)tiles * (xcd + 1) / 8)) return;
+  const int g = u / (8 * a.tv), gr = min(8, a.tr - 8 * g), in = u - 8 * a.tv * g;
+  const int tr = 8 * g + in % gr, tv = in / gr;
+  // A stage: [32 entries or rows][part][piece], entries first. Blocks past the operands'
+  // last read the last (their results are not used).
+  const int64_t bw = ((int64_t)a.V + 31) / 32 - 1, bx = (a.rows + 31) / 32 - 1;
+  const uint16_t* from[(FW + FX) / 4];
+#pragma unroll
+  for (int k = 0; k < (FW + FX) / 4; ++k) {
+    const int f = w + 4 * k;
+    const int64_t blk = f < FW ? min((int64_t)tv * FW + f, bw) : min((int64_t)tr * FX + f - FW, bx);
+    from[k] = (f < FW ? a.w : a.x) + blk * a.ke * 1024 + lane * 8;
+  }
+  auto stage = [&](int t, int b) {
+#pragma unroll
+    for (int k = 0; k < (FW + FX) / 4; ++k) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) pa_copy16(from[k] + (int64_t)t * 1024 + p * 512, &ls[b][(w + 4 * k) * 1024 + p * 512]);
+    }
+  };
+  pa_f16 acc[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = pa_f16{};
+  stage(0, 0);
+  stage(1, 1);  // (ke is even)
+  const int row0 = pa_piece(lane, 0) * 8, row1 = pa_piece(lane, 1) * 8;
+  int b = 0;
+  for (int t = 0; t < a.ke; ++t) {
+    if (t + 1 < a.ke) pa_arrived_but<(FW + FX) / 2>();
+    else pa_arrived();
+    if (t + 2 < a.ke) stage(t + 2, b == 0 ? 2 : b - 1);
+    const uint16_t* p = ls[b] + (t & 1 ? row1 : row0);
+    auto frag = [&](int f) {
+      return PaFrag{*reinterpret_cast<const pa_h8*>(p + f * 1024), *reinterpret_cast<const pa_h8*>(p + f * 1024 + 512)};
+    };
+    PaFrag fw[2], fx[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) fw[i] = frag(2 * w + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fx[j] = frag(FW + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i][j] = pa_mfma(fw[i].l, fx[j].h, acc[i][j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i][j] = pa_mfma(fw[i].h, fx[j].l, acc[i][j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i][j] = pa_mfma(fw[i].h, fx[j].h, acc[i][j]);
+    b = b == 2 ? 0 : b + 1;
+  }
+  // Lane (li, hf): rows 32 j + li, entries 32 i + 8 (r / 4) + 4 hf + r % 4 of the wave's 64.
+  const int v0 = tv * VH_LX_TV + 64 * w + 4 * hf;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int v = v0 + 32 * i + 8 * y;  // (the exponents are padded to whole blocks of 32)
+      const int4 e = v < a.V ? *reinterpret_cast<const int4*>(a.we + v) : int4{0, 0, 0, 0};
+      const int ev[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i][j][4 * y + k] = pa_ldexp(acc[i][j][4 * y + k], ev[k]);
+    }
+  const bool whole = tv * VH_LX_TV + VH_LX_TV <= a.V;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = (int64_t)tr * VH_LX_TR + 32 * j + li;
+    const bool live = r < a.rows;
+    const int ex = live ? a.xe[r] - 2 * PA_E : 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[i][j][k] = pa_ldexp(acc[i][j][k], ex);
+    if (a.z && live) {
+      float* z = a.z + r * a.ld;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int v = v0 + 32 * i + 8 * y;
+          if (v < a.V)  // (ld is a multiple of 4: the row's last unit is inside it)
+            *reinterpret_cast<pa_f4*>(z + v) =
+                pa_f4{acc[i][j][4 * y], acc[i][j][4 * y + 1], acc[i][j][4 * y + 2], acc[i][j][4 * y + 3]};
+        }
+    }
+    if (!a.part) continue;
+    const float t = live ? a.targets[r] : a.ignore;
+    const int32_t at = t != a.ignore ? checked_index(t, a.V) : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int v = v0 + 32 * i + 8 * (k >> 2) + (k & 3);
+        if (v == at) a.zt[r] = acc[i][j][k];
+        if (!whole && v >= a.V) acc[i][j][k] = -INFINITY;
+        m = fmaxf(m, acc[i][j][k]);
+      }
+    m = pa_max_halves(m);
+    const float mb = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f((acc[i][j][k] - mb) * PA_LOG2E);
+    s = pa_sum_halves(s);
+    if (hf == 0) {
+      red[w][32 * j + li][0] = m;
+      red[w][32 * j + li][1] = s;
+    }
+  }
+  if (!a.part) return;
+  __syncthreads();
+  const int64_t r = (int64_t)tr * VH_LX_TR + threadIdx.x;
+  if (threadIdx.x >= VH_LX_TR || r >= a.rows) return;
+  float m = red[0][threadIdx.x][0];
+#pragma unroll
+  for (int k = 1; k < 4; ++k) m = fmaxf(m, red[k][threadIdx.x][0]);
+  const float mb = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s += red[k][threadIdx.x][1] * expf(red[k][threadIdx.x][0] - mb);
+  *reinterpret_cast<float2*>(a.part + (r * a.tv + tv) * 2) = make_float2(m, s);
+}
+
+// A row's max and sum of exp from its tiles', in a fixed order, and its loss term. A wave
+// per row.
+VH_DEV void lx_finish_impl(const LxFinishArgs& a) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (r >= a.rows) return;
+  const float2* p = reinterpret_cast<const float2*>(a.part) + r * a.tv;
+  float m = -INFINITY;
+  for (int t = lane; t < a.tv; t += 64) m = fmaxf(m, p[t].x);
+  m = group_max<64>(m);
+  const float mb = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+  for (int t = lane; t < a.tv; t += 64) s += p[t].y * expf(p[t].x - mb);
+  s = group_sum<64>(s);
+  if (m == -INFINITY) s = NAN;  // exp(-inf - -inf)
+  if (lane) return;
+  const float t = a.targets[r];
+  const bool counted = t != a.ignore && checked_index(t, a.V) >= 0;
+  *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(m, s);
+  a.row_loss[r] = counted ? m + logf(s) - a.zt[r] : 0.0f;
 }

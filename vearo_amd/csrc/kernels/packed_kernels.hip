@@ -33,3 +33,6 @@ extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_stats(LxArgs a) { l
 extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_grad(LxArgs a) { lx_row_impl<false, true>(a); }
 extern "C" __global__ void __launch_bounds__(LX_BLOCK) vh_lx_stats_grad(LxArgs a) { lx_row_impl<true, true>(a); }
 extern "C" __global__ void __launch_bounds__(1024) vh_lx_loss(LxLossArgs a) { lx_loss_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_lx_split(LxSplitArgs a) { lx_split_impl(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) vh_lx_logits(LxLogitArgs a) { lx_logits_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_lx_finish(LxFinishArgs a) { lx_finish_impl(a); }

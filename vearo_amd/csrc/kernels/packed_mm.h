@@ -235,6 +235,14 @@ VH_DEV void pa_arrived() {
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
 }
+// The same while the last N copies of each wave may still be on their way.
+template <int N>
+VH_DEV void pa_arrived_but() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 // A tile's exponent, the same for all lanes, by the scalar unit: a vector load would wait
 // for the copies in flight before it. (Constant memory here: the prepare launch wrote it.)
 typedef const __attribute__((address_space(4))) int32_t* PaInfo;

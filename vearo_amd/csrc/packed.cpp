@@ -236,20 +236,44 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
 }
 
 // ------------------------------------------------- cross-entropy of a linear layer --
-constexpr size_t kLxPieceBytes = size_t(256) << 20;
+constexpr size_t kLxPieceBytes = size_t(1) << 30;
 int64_t lx_ld(int64_t V) { return (V + 3) / 4 * 4; }
-// Rows per piece: whole 256-row product tiles within kLxPieceBytes, one at least.
-int64_t lx_rows(int64_t R, int64_t V) {
-  const int64_t fit = (int64_t)(kLxPieceBytes / (sizeof(float) * (size_t)lx_ld(V))) / 256 * 256;
-  return std::min<int64_t>(R, std::max<int64_t>(fit, 256));
+// Logits by the f16 parts (vh_lx_logits) from this many multiply-adds on; below, the
+// splitting of both operands costs more than the products.
+constexpr double kLxLogits = 268435456.0;
+bool lx_by_parts(int64_t R, int64_t D, int64_t V) { return (double)R * (double)D * (double)V >= kLxLogits; }
+// Rows per piece: pieces of even size in whole 256-row product tiles, within kLxPieceBytes
+// of logits (one tile at least). The gradient's products want many rows: at [16384, 50257],
+// D = 768, pieces of 256 MB take 23.9 ms, 512 MB 22.0, 1 GB 20.7, 2 GB 20.0. A forward that
+// keeps no logits at all is one piece.
+int64_t lx_rows(int64_t R, int64_t D, int64_t V, bool backward) {
+  if (!backward && lx_by_parts(R, D, V)) return R;
+  const int64_t fit = std::max<int64_t>((int64_t)(kLxPieceBytes / (sizeof(float) * (size_t)lx_ld(V))) / 256 * 256, 256);
+  return std::min<int64_t>(R, cdiv(cdiv(R, cdiv(R, fit)), 256) * 256);
 }
 struct LxScratch {
-  size_t z, row_loss, inv, total;
-  LxScratch(int64_t R, int64_t V) {
-    z = 0;
-    row_loss = align256(sizeof(float) * (size_t)(lx_rows(R, V) * lx_ld(V)));
-    inv = row_loss + align256(sizeof(float) * (size_t)R);
-    total = inv + 256;
+  size_t z, row_loss, inv, stats, xf, xe, wf, we, part, zt, total;
+  LxScratch(int64_t R, int64_t D, int64_t V, bool backward) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t p = at;
+      at += align256(bytes);
+      return p;
+    };
+    const bool parts = lx_by_parts(R, D, V);
+    const int64_t rows = lx_rows(R, D, V, backward);
+    z = take(parts && !backward ? 0 : sizeof(float) * (size_t)(rows * lx_ld(V)));
+    row_loss = take(sizeof(float) * (size_t)R);
+    inv = take(256);
+    stats = take(backward ? 2 * sizeof(float) * (size_t)R : 0);  // (of a call that returns none)
+    const size_t ke = (size_t)cdiv(D, 32) * 2, xb = (size_t)cdiv(rows, 32), wb = (size_t)cdiv(V, 32);
+    xf = take(parts ? xb * ke * 2048 : 0);
+    xe = take(parts ? xb * 32 * sizeof(int32_t) : 0);
+    wf = take(parts ? wb * ke * 2048 : 0);
+    we = take(parts ? wb * 32 * sizeof(int32_t) : 0);
+    part = take(parts ? 2 * sizeof(float) * (size_t)(rows * cdiv(V, VH_LX_TV)) : 0);
+    zt = take(parts ? sizeof(float) * (size_t)rows : 0);
+    total = at;
   }
 };
 
@@ -300,24 +324,44 @@ int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes,
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(s, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
     return fail(VH_ERR_UNSUPPORTED, f + ": cannot run under graph capture");
-  const LxScratch lay(c.R, c.V);
+  const LxScratch lay(c.R, c.D, c.V, c.backward);
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   char* base = static_cast<char*>(sc.p);
-  float* z = reinterpret_cast<float*>(base + lay.z);
-  float* row_loss = reinterpret_cast<float*>(base + lay.row_loss);
-  float* inv = reinterpret_cast<float*>(base + lay.inv);
-  const int64_t ld = lx_ld(c.V), piece = lx_rows(c.R, c.V);
-  VH_TRY(launch("vh_lx_count", 1, 1, 1, 1024, s,
-                LxCountArgs{c.targets, inv, vh_rt::error_record(), c.R, (int32_t)c.V, c.ignore}));
-  const char* kernel = c.forward ? (c.backward ? "vh_lx_stats_grad" : "vh_lx_stats") : "vh_lx_grad";
+  auto at = [&](size_t off) { return reinterpret_cast<float*>(base + off); };
+  auto frags = [&](size_t off) { return reinterpret_cast<uint16_t*>(base + off); };
+  auto exps = [&](size_t off) { return reinterpret_cast<int32_t*>(base + off); };
+  float *z = at(lay.z), *row_loss = at(lay.row_loss), *inv = at(lay.inv);
+  float* stats = c.stats ? c.stats : at(lay.stats);
+  const int64_t ld = lx_ld(c.V), piece = lx_rows(c.R, c.D, c.V, c.backward);
+  const bool parts = lx_by_parts(c.R, c.D, c.V);
+  const int32_t V = (int32_t)c.V, ke = (int32_t)(cdiv(c.D, 32) * 2);
+  auto split = [&](const float* p, int64_t stride, int64_t rows, size_t f, size_t e) {
+    const LxSplitArgs a{p, frags(f), exps(e), rows, stride, (int32_t)c.D, ke,
+                        aligned16(p) && stride % 4 == 0 && c.D % 4 == 0};
+    return launch("vh_lx_split", cdiv(rows, 32), 1, 1, 256, s, a);
+  };
+  VH_TRY(launch("vh_lx_count", 1, 1, 1, 1024, s, LxCountArgs{c.targets, inv, vh_rt::error_record(), c.R, V, c.ignore}));
+  if (parts) VH_TRY(split(c.w, c.ldw, c.V, lay.wf, lay.we));
   for (int64_t r = 0; r < c.R; r += piece) {
     const int64_t rows = std::min(piece, c.R - r);
-    const float* x = c.x + r * c.ldx;
-    VH_TRY(lx_product(rows, c.V, c.D, x, c.ldx, 1, c.w, 1, c.ldw, z, ld, false, s));
-    VH_TRY(launch(kernel, rows, 1, 1, 512, s,
-                  LxArgs{z, c.targets + r, c.grad_out, inv, c.stats ? c.stats + 2 * r : nullptr,
-                         c.forward ? row_loss + r : nullptr, rows, ld, (int32_t)c.V, c.ignore}));
+    const float *x = c.x + r * c.ldx, *t = c.targets + r;
+    float* st = stats + 2 * r;
+    if (parts) {
+      const int32_t tv = (int32_t)cdiv(c.V, VH_LX_TV), tr = (int32_t)cdiv(rows, VH_LX_TR);
+      VH_TRY(split(x, c.ldx, rows, lay.xf, lay.xe));
+      const LxLogitArgs a{frags(lay.wf), exps(lay.we), frags(lay.xf), exps(lay.xe), t, c.forward ? at(lay.part) : nullptr,
+                          at(lay.zt), c.backward ? z : nullptr, rows, ld, V, ke, tv, tr, c.ignore};
+      VH_TRY(launch("vh_lx_logits", cdiv((int64_t)tv * tr, 8) * 8, 1, 1, 256, s, a));
+      if (c.forward)
+        VH_TRY(launch("vh_lx_finish", cdiv(rows, 4), 1, 1, 256, s,
+                      LxFinishArgs{at(lay.part), at(lay.zt), t, st, row_loss + r, rows, V, tv, c.ignore}));
+    } else {
+      VH_TRY(lx_product(rows, c.V, c.D, x, c.ldx, 1, c.w, 1, c.ldw, z, ld, false, s));
+    }
+    const char* kernel = parts || !c.forward ? "vh_lx_grad" : c.backward ? "vh_lx_stats_grad" : "vh_lx_stats";
+    if (c.backward || !parts)
+      VH_TRY(launch(kernel, rows, 1, 1, 512, s, LxArgs{z, t, c.grad_out, inv, st, row_loss + r, rows, ld, V, c.ignore}));
     if (!c.backward) continue;
     VH_TRY(lx_product(rows, c.D, c.V, z, ld, 1, c.w, c.ldw, 1, c.dx + r * c.lddx, c.lddx, false, s));
     VH_TRY(lx_product(c.V, c.D, rows, z, 1, ld, x, c.ldx, 1, c.dw, c.lddw, r > 0, s));
@@ -469,9 +513,9 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
   return launch("vh_pa_dq_" + dp, a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }
 
-size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t V) {
-  if (R <= 0 || V <= 0) return 0;
-  return LxScratch(R, V).total;
+size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t D, int64_t V, int backward) {
+  if (R <= 0 || D <= 0 || V <= 0) return 0;
+  return LxScratch(R, D, V, backward != 0).total;
 }
 
 int vh_linear_cross_entropy_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,

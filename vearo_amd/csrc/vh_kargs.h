@@ -503,6 +503,8 @@ struct PaArgs {
 };
 
 // Cross-entropy of a linear layer in pieces of rows (kernels/linxent.h).
+#define VH_LX_TV 256  // vocabulary entries and rows of one product tile
+#define VH_LX_TR 128
 struct LxArgs {
   float* z;              // [rows, ld] logits of the piece; the backward's become their gradient
   const float* targets;  // of the piece
@@ -527,4 +529,37 @@ struct LxLossArgs {
   const float* inv;
   float* loss;
   int64_t R;
+};
+// Rows of a matrix as two f16 parts under a power of two per row, in fragments.
+struct LxSplitArgs {
+  const float* x;
+  uint16_t* frag;  // [32 rows][16 elements][part][64 pieces of 8]
+  int32_t* exp;    // [rows padded to 32] exponents
+  int64_t rows, ld;
+  int32_t D, ke;   // ke: fragments along a row, a multiple of 2
+  int32_t vec;
+};
+struct LxLogitArgs {
+  const uint16_t* w;     // fragments and exponents of the vocabulary entries, and of the rows
+  const int32_t* we;
+  const uint16_t* x;
+  const int32_t* xe;
+  const float* targets;  // of the rows
+  float* part;           // [rows][tiles of entries][2] max, sum of exp; null: not wanted
+  float* zt;             // [rows] the target's logit (with part)
+  float* z;              // [rows, ld] logits, or null
+  int64_t rows, ld;
+  int32_t V, ke;
+  int32_t tv, tr;        // tiles of entries, of rows
+  float ignore;
+};
+struct LxFinishArgs {
+  const float* part;
+  const float* zt;
+  const float* targets;
+  float* stats;
+  float* row_loss;
+  int64_t rows;
+  int32_t V, tv;
+  float ignore;
 };
