@@ -169,8 +169,8 @@ VH_DEV void rope_fwd_impl(const RopeArgs& a) {
   }
 }
 
-// Teams walk the tokens grid-stride (a fixed grid: the weight gradients' grouping
-// depends on the sizes alone); each lane sums its elements' weight gradients over
+// Grid: (token groups, head groups of a.heads_per). Teams walk the tokens grid-stride (a
+// grid of the sizes alone, and so the weight gradients' grouping); each lane sums its elements' weight gradients over
 // its tokens and heads, the workgroup's teams are added in order, and vh_col_reduce
 // adds the workgroups.
 template <int VW, int LPR, int NS>
@@ -187,17 +187,19 @@ VH_DEV void rope_bwd_impl(const RopeArgs& a) {
     for (int i = 0; i < 2; ++i) {
       float wa[NS][VW], wb[NS][VW];
       tm.load(a.w[i], a.D, wa, wb);
-      for (int h = 0; h < a.H[i]; h += 2) {  // two heads' loads in flight
+      const int lo = max(0, (int)blockIdx.y * a.heads_per - (i ? a.H[0] : 0));
+      const int hi = min(a.H[i], ((int)blockIdx.y + 1) * a.heads_per - (i ? a.H[0] : 0));
+      for (int h = lo; h < hi; h += 2) {  // two heads' loads in flight
         float x2a[2][NS][VW], x2b[2][NS][VW], g2a[2][NS][VW], g2b[2][NS][VW];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const int hb = min(h + b, a.H[i] - 1);
+          const int hb = min(h + b, hi - 1);
           tm.load(a.x[i] + t * a.xt[i] + hb * a.xh[i], a.D, x2a[b], x2b[b]);
           tm.load(a.dy[i] + t * a.dt[i] + hb * a.dh[i], a.D, g2a[b], g2b[b]);
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          if (h + b >= a.H[i]) break;
+          if (h + b >= hi) break;
           auto &xa = x2a[b], &xb = x2b[b], &ga = g2a[b], &gb = g2b[b];
           const float ss = group_sum<LPR>(rope_dot<NS, VW>(xa, xb, xa, xb));
           const float r = 1.0f / sqrtf(ss / fd + a.eps);
@@ -240,7 +242,7 @@ VH_DEV void rope_bwd_impl(const RopeArgs& a) {
     for (int d = threadIdx.x; d < a.D; d += 256) {
       float s = acc[0][d];
       for (int k = 1; k < TEAMS; ++k) s += acc[k][d];
-      a.part[((int64_t)blockIdx.x * 2 + i) * a.D + d] = s;
+      a.part[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + i) * a.D + d] = s;
     }
   }
 }

@@ -391,7 +391,8 @@ int vh_qk_norm_rope_fwd(const float* q, const vh_layout* ql, const float* k, con
   VH_TRY(vh_rt::require_init());
   rope_out(&a, qo, qol, ko, kol);
   const RopeCfg c = rope_cfg(hq.D, rotary, vec && rows16(qo, qol) && rows16(ko, kol));
-  a.heads_per = hq.T * c.lpr * cdiv(H, 8) < (int64_t(1) << 19) ? 4 : 8;
+  // Heads per workgroup: two where tokens are few, else eight (the angles are formed once for them).
+  a.heads_per = hq.T * c.lpr < (int64_t(1) << 16) ? 2 : 8;
   return launch("vh_rope_fwd" + c.suffix(), cdiv(hq.T, 256 / c.lpr), cdiv(H, a.heads_per), 1, 256,
                 vh_rt::stream_of(stream), a);
 }
@@ -435,8 +436,13 @@ int vh_qk_norm_rope_bwd(const float* q, const vh_layout* ql, const float* k, con
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, vh_qk_norm_rope_bwd_scratch_bytes(hq.T, hq.D)));
   a.part = static_cast<float*>(sc.p);
-  VH_TRY(launch("vh_rope_bwd" + c.suffix(), blocks, 1, 1, 256, s, a));
-  ColReduceArgs r{a.part, dwq, dwk, (int32_t)blocks, a.D, 2};
+  // Few tokens: their heads over several workgroups, two at least each (the scratch holds a
+  // row of sums for every fourth token).
+  const int64_t H = hq.H + hk.H, room = std::min<int64_t>(cdiv(hq.T, 4), kRopeBwdBlocks) / blocks;
+  a.heads_per = (int32_t)(blocks >= 256 ? H : std::max<int64_t>(2, cdiv(H, std::max<int64_t>(room, 1))));
+  const int64_t groups = cdiv(H, a.heads_per);
+  VH_TRY(launch("vh_rope_bwd" + c.suffix(), blocks, groups, 1, 256, s, a));
+  ColReduceArgs r{a.part, dwq, dwk, (int32_t)(blocks * groups), a.D, 2};
   return launch("vh_col_reduce", cdiv(hq.D, VH_COLR_COLS), 2, 1, VH_COLR_COLS * 16, s, r);
 }
 
