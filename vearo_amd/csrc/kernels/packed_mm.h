@@ -53,7 +53,9 @@ typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
 #define PA_SHIFT 3
 #define PA_PV 11           // dV's P is held at 2^11, below 2^14 with the shift
 #define PA_LOG2E 1.4426950408889634f
+#define PA_LOG2E_LO 1.9259629911266175e-8f  // log2(e) - PA_LOG2E
 #define PA_LN2 0.6931471805599453f
+#define PA_LN2_LO -1.904654299957768e-9f
 
 // Two values -> the f16 pairs of their parts.
 VH_DEV void pa_split2(float x0, float x1, uint32_t& h, uint32_t& l) {
@@ -168,7 +170,7 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
     const int64_t tok = (int64_t)h * a.T + sp.start + i;
     if ((tid & 3) == 0) {
       float* s = a.stat + at * 128 + (row >> 5) * 64 + (row & 31);
-      s[0] = live ? a.lse[tok] * PA_LOG2E - (float)PA_PV : INFINITY;
+      s[0] = live ? fmaf(a.lse[tok], PA_LOG2E, fmaf(a.lse[tok], PA_LOG2E_LO, -(float)PA_PV)) : INFINITY;
       s[32] = live ? dl : 0.0f;
       if (live) a.delta[tok] = dl;
     }
@@ -503,7 +505,7 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   const float inv = 1.0f / l;
   pa_store<DB>(a.out + tok * a.out_t + h * a.out_h, a.out_vec, a.D, o,
                [&](float v) { return pa_ldexp(v * inv, ev - PA_E); });
-  if (hf == 0) a.lse[(int64_t)h * a.T + tok] = (m - (float)PA_E) * PA_LN2 + logf(l);
+  if (hf == 0) a.lse[(int64_t)h * a.T + tok] = fmaf(m, PA_LN2, fmaf(m, PA_LN2_LO, logf(pa_ldexp(l, -PA_E))));
 }
 
 // -------------------------------------------------------------------- backward --
@@ -565,7 +567,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
     return;
   }
   const int64_t tok = (int64_t)sp.start + i;
-  const float lse = live ? a.lse[(int64_t)h * a.T + tok] * PA_LOG2E : 0.0f;
+  const float le = live ? a.lse[(int64_t)h * a.T + tok] : 0.0f, lse = fmaf(le, PA_LOG2E, le * PA_LOG2E_LO);
   const float dl = live ? a.delta[(int64_t)h * a.T + tok] : 0.0f;
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
   const float cs = a.scale * PA_LOG2E;
