@@ -39,7 +39,7 @@ def test_lengths(vh, lens, causal):
     run_and_check(vh, lens, 4, 2, 64, causal)
 
 
-@pytest.mark.parametrize("D", [1, 2, 7, 16, 31, 32, 33, 40, 64, 65, 80, 96, 112, 127, 128, 129, 160, 256])
+@pytest.mark.parametrize("D", [1, 2, 7, 16, 31, 32, 33, 40, 64, 65, 80, 96, 112, 127, 128, 129, 160, 192, 193, 255, 256])
 @pytest.mark.parametrize("causal", [True, False])
 def test_head_sizes(vh, D, causal):
     run_and_check(vh, [150, 1, 70], 2, 1, D, causal, seed=D)

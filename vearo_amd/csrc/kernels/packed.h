@@ -1,5 +1,5 @@
 // packed.h -- attention over packed sequences with grouped heads, forward and
-// backward: the tables, and the row kernels that take any head size and any values.
+// backward: the tables, and the row forms that take any values.
 //
 // T tokens hold n sequences one behind the other, sequence s the tokens
 // starts[s] .. starts[s + 1] - 1; query head h reads key head h / (Hq / Hk). Within a
@@ -123,18 +123,12 @@ VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
   }
 }
 
-VH_DEV void pa_plan_impl(const PaArgs& a) {
-  __shared__ PaFind f;
-  pa_tables(a, blockIdx.x, f);
-}
-
 // ------------------------------------------------------------ row kernels --
 // A wave per row, keys over its lanes for the scores, elements over its lanes for
 // the products. Scores are formed again in each pass instead of kept, so a row may
 // have any length. f32 arithmetic throughout, element by element, nothing masked
-// ever touched. These carry head sizes past 128 and, inside the matrix kernels,
-// blocks whose values those cannot hold; a row costs its dot products (about a
-// tenth of the vector units' rate, each lane reading its own key's row).
+// ever touched. These carry the blocks whose values the matrix kernels (packed_mm.h)
+// cannot hold, about a hundred times slower: each lane reads a key's row by itself.
 
 // An LDS row of up to 256 elements that the wave alone reads and writes.
 VH_DEV void pa_row_to_lds(float* l, const float* p, int D) {
@@ -234,9 +228,8 @@ VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float*
   float* ok = a.dk + tok * a.dk_t + hk * a.dk_h;
   float* ov = a.dv + tok * a.dv_t + hk * a.dv_h;
   if (a.parts > 1) {
-    const int dp = (a.D + 31) / 32 * 32;
-    ok = a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * dp;
-    ov = ok + (int64_t)a.T * a.k.H * dp;
+    ok = a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * a.DP;
+    ov = ok + (int64_t)a.T * a.k.H * a.DP;
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
@@ -256,30 +249,5 @@ VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, float (*l)[2][VH_P
     if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l[w][0]);
     if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l[w][0], l[w][1]);
     if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l[w][0], l[w][1], h0, h1, part);
-  }
-}
-// Grid: (blocks, heads: of q, or of k for dk and dv).
-template <int MODE>
-VH_DEV void pa_rows_impl(const PaArgs& a) {
-  __shared__ float l[4][2][VH_PA_MAX_D];
-  if ((int)blockIdx.x >= a.head->nblocks) return;
-  const int G = a.q.H / a.k.H;
-  pa_rows<MODE>(a, blockIdx.y, a.blocks[blockIdx.x], l, blockIdx.y * G, (blockIdx.y + 1) * G);
-}
-
-// delta[h][t] = sum over d of dout * out for every row of the sequences, a wave per row
-// of 64-row tile blockIdx.x and head blockIdx.y.
-VH_DEV void pa_delta_impl(const PaArgs& a) {
-  if ((int)blockIdx.x >= a.head->ntiles) return;
-  const PaSpan sp = a.tiles[blockIdx.x];
-  const int lane = threadIdx.x & 63, h = blockIdx.y;
-  for (int i = sp.row0 + (threadIdx.x >> 6); i < min(sp.len, sp.row0 + 64); i += 4) {
-    const int64_t tok = (int64_t)sp.start + i;
-    const float* o = a.o.p + tok * a.o.st + h * a.o.sh;
-    const float* g = a.g.p + tok * a.g.st + h * a.g.sh;
-    float s = 0.0f;
-    for (int d = lane; d < a.D; d += 64) s = fmaf(o[d], g[d], s);
-    s = group_sum<64>(s);
-    if (lane == 0) a.delta[(int64_t)h * a.T + tok] = s;
   }
 }

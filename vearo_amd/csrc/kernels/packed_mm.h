@@ -1,5 +1,4 @@
-// packed_mm.h -- attention over packed sequences on the f16 matrix instruction, head
-// sizes up to 128: f32 products carried by two f16 parts per operand.
+// packed_mm.h -- attention over packed sequences on the f16 matrix instruction: f32 products carried by two f16 parts per operand.
 //
 // An f32 value scaled to |x| < 2^15 is h + l + r, h = f16(x), l = f16(x - h), with
 // |r| <= 2^-22 |x| down to 2^-18 of the largest value the scale was made for and
@@ -623,13 +622,14 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
 // rows for S and dO V^T and by columns for dV and dK. Its accumulators and resident rows
 // leave no registers for a second step's S: what overlaps is the exp of S with dO V^T and
 // dS with dV. Where the blocks are few the query heads are divided over a.parts workgroups,
-// whose sums pa_join adds in order.
-template <int DP, int NW>
+// whose sums pa_join adds in order. HALVES 2: a workgroup forms one half of dk's and dv's
+// elements, all of which are too many registers past 128.
+template <int DP, int NW, int HALVES>
 VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
-  constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
+  constexpr int KS = DP / 16, DB = DP / 32 / HALVES, SUB = 64 * DP;
   __shared__ __attribute__((aligned(1024))) uint16_t lq[2][SUB], lg[2][SUB];
   __shared__ __attribute__((aligned(1024))) float lst[2][64];  // a step's 32 log2-lse and 32 delta
-  const int H = a.k.H * a.parts, id = blockIdx.x;
+  const int H = a.k.H * a.parts, half = blockIdx.x % HALVES, id = blockIdx.x / HALVES;
   PaSpan sp = a.blocks[id / H];
   if (id >= a.head->nblocks * H) return;
   // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
@@ -672,7 +672,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   const bool slow_q = rq.any_slow(topq), slow_g = rg.any_slow(topg);
   if (slow_q || slow_g) {
     pa_arrived();
-    pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
+    if (half == 0) pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
     return;
   }
   const float cs = a.scale * PA_LOG2E;
@@ -720,7 +720,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
     for (int u = 0; u < 2; ++u) {
       const PaFrag f = pa_split8([&](int y) { return s[8 * u + y] * ps; });
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(fg.cols(b, db, u), f, dv[db]);
+      for (int db = 0; db < DB; ++db) pa_mma(fg.cols(b, half * DB + db, u), f, dv[db]);
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
@@ -733,7 +733,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
     for (int u = 0; u < 2; ++u) {
       const PaFrag f = pa_split8([&](int y) { return s[8 * u + y] * gs; });
 #pragma unroll
-      for (int db = 0; db < DB; ++db) pa_mma(fq.cols(b, db, u), f, dk[db]);
+      for (int db = 0; db < DB; ++db) pa_mma(fq.cols(b, half * DB + db, u), f, dk[db]);
     }
   }
   if (j >= sp.len) return;
@@ -741,8 +741,9 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   const bool whole = a.parts == 1;
   float* const to_k = whole ? a.dk + tok * a.dk_t + hk * a.dk_h : a.join + (((int64_t)part * 2 * a.T + tok) * a.k.H + hk) * DP;
   float* const to_v = whole ? a.dv + tok * a.dv_t + hk * a.dv_h : a.join + ((((int64_t)part * 2 + 1) * a.T + tok) * a.k.H + hk) * DP;
-  pa_store<DB>(to_k, whole ? a.dk_vec : 1, whole ? a.D : DP, dk, [&](float y) { return pa_ldexp(y * a.scale, topq - PA_E - PA_PV - g); });
-  pa_store<DB>(to_v, whole ? a.dv_vec : 1, whole ? a.D : DP, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
+  const int d0 = half * DB * 32, D = (whole ? a.D : DP) - d0;
+  pa_store<DB>(to_k + d0, whole ? a.dk_vec : 1, D, dk, [&](float y) { return pa_ldexp(y * a.scale, topq - PA_E - PA_PV - g); });
+  pa_store<DB>(to_v + d0, whole ? a.dv_vec : 1, D, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
 }
 
 // dk and dv of each token in a sequence: the parts' sums, in order. Grid: (tiles,

@@ -117,18 +117,15 @@ void rope_out(RopeArgs* a, float* yq, const vh_layout* qol, float* yk, const vh_
 // ------------------------------------------------------------ packed attention --
 int64_t pa_units(int64_t T, int64_t n, int64_t rows) { return T / rows + n; }
 
-// Head sizes up to kPaMatrixD run on the matrix kernels (padded to a multiple of 32), whose
-// workgroups own blocks of 128 rows; larger ones on the row kernels.
-constexpr int64_t kPaMatrixD = 128;
-int pa_padded(int64_t D) { return (int)(cdiv(D, 32) * 32); }
-int pa_block_rows(int64_t D) { return D <= kPaMatrixD ? 128 : 64; }
+constexpr int kPaBlockRows = 128;  // rows of a workgroup
+// The kernels' head sizes.
+int pa_padded(int64_t D) { return D <= 128 ? (int)cdiv(D, 32) * 32 : (int)cdiv(D, 64) * 64; }
 
 // Workgroups that share a key head's query heads in dk and dv: as many as bring the blocks
 // to kPaJoinBlocks, where a block's first keys meet every query after them. [8192] tokens, 16
 // query heads on 2 of 128: 128 workgroups take 7.2 ms for what 1024 do in PLACEHOLDER.
 constexpr int64_t kPaJoinBlocks = 1024;
-int pa_parts(int64_t T, int64_t Hq, int64_t Hk, int64_t D) {
-  if (D > kPaMatrixD) return 1;
+int pa_parts(int64_t T, int64_t Hq, int64_t Hk) {
   const int64_t G = Hq / Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk)));
   return (int)cdiv(G, per);
 }
@@ -146,14 +143,13 @@ struct PaScratch {
     const size_t units = (size_t)pa_units(T, seqs, 64);
     head = take(sizeof(PaHead));
     tiles = take(sizeof(PaSpan) * units);
-    blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, seqs, pa_block_rows(D)));
+    blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, seqs, kPaBlockRows));
     delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
-    const bool mm = D <= kPaMatrixD;
-    stat = take(mm && backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
-    const int parts = pa_parts(T, Hq, Hk, D);
+    stat = take(backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
+    const int parts = pa_parts(T, Hq, Hk);
     join = take(backward && parts > 1 ? sizeof(float) * 2 * (size_t)(parts * T * Hk * pa_padded(D)) : 0);
     for (int i = 0; i < 4; ++i) {
-      const size_t tiles_h = mm && (backward || i < 2) ? units * (size_t)(i < 2 ? Hk : Hq) : 0;
+      const size_t tiles_h = backward || i < 2 ? units * (size_t)(i < 2 ? Hk : Hq) : 0;
       n[i] = take(tiles_h * 256 * (size_t)pa_padded(D));
       info[i] = take(tiles_h * sizeof(int32_t));
     }
@@ -199,7 +195,8 @@ int pa_check(const std::string& f, const float* q, const vh_layout* ql, const fl
   a.n = (int32_t)n;
   a.T = (int32_t)T;
   a.D = (int32_t)D;
-  a.block_rows = pa_block_rows(D);
+  a.DP = pa_padded(D);
+  a.block_rows = kPaBlockRows;
   a.max_tiles = (int32_t)std::min<int64_t>(pa_units(T, n, 64), INT32_MAX);
   a.max_blocks = (int32_t)std::min<int64_t>(pa_units(T, n, a.block_rows), INT32_MAX);
   a.causal = causal != 0;
@@ -207,8 +204,7 @@ int pa_check(const std::string& f, const float* q, const vh_layout* ql, const fl
   return VH_OK;
 }
 
-// Places the workspace and, for the matrix kernels, launches the prepare step: the
-// tables and the streams' fragments.
+// Places the workspace and launches the prepare step: the tables and the streams' fragments.
 int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStream_t s) {
   PaArgs& a = c->a;
   char* p = static_cast<char*>(base);
@@ -218,12 +214,8 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
   a.delta = reinterpret_cast<float*>(p + l.delta);
   a.stat = reinterpret_cast<float*>(p + l.stat);
   a.join = reinterpret_cast<float*>(p + l.join);
-  a.parts = backward ? pa_parts(c->q.T, c->q.H, c->k.H, c->q.D) : 1;
+  a.parts = backward ? pa_parts(c->q.T, c->q.H, c->k.H) : 1;
   a.grad = -1;
-  if (c->q.D > kPaMatrixD) {
-    VH_TRY(launch("vh_pa_plan", std::max(a.max_tiles, a.max_blocks), 1, 1, 256, s, a));
-    return backward ? launch("vh_pa_delta", a.max_tiles, c->q.H, 1, 256, s, a) : VH_OK;
-  }
   const PaTensor t[4] = {a.k, a.v, a.q, a.g};
   const int streams = backward ? 4 : 2;
   for (int i = 0; i < streams; ++i) {
@@ -231,7 +223,7 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
                            i < 2 ? VH_PA_SPAN_KV : VH_PA_SPAN_Q};
   }
   if (backward) a.grad = 3;
-  return launch("vh_pa_prep_" + std::to_string(pa_padded(c->q.D)), a.max_tiles, backward ? c->q.H : c->k.H, streams, 256,
+  return launch("vh_pa_prep_" + std::to_string(a.DP), a.max_tiles, backward ? c->q.H : c->k.H, streams, 256,
                 s, a);
 }
 
@@ -469,8 +461,7 @@ int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k,
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   VH_TRY(pa_prepare(&c, lay, sc.p, false, s));
-  if (c.q.D > kPaMatrixD) return launch("vh_pa_rows_fwd", a.max_blocks, c.q.H, 1, 256, s, a);
-  return launch("vh_pa_fwd_" + std::to_string(pa_padded(c.q.D)), a.max_blocks * c.q.H, 1, 1, 256, s, a);
+  return launch("vh_pa_fwd_" + std::to_string(a.DP), a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }
 
 int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
@@ -509,12 +500,8 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   VH_TRY(pa_prepare(&c, lay, sc.p, true, s));
-  if (c.q.D > kPaMatrixD) {
-    VH_TRY(launch("vh_pa_rows_dq", a.max_blocks, c.q.H, 1, 256, s, a));
-    return launch("vh_pa_rows_dkdv", a.max_blocks, c.k.H, 1, 256, s, a);
-  }
-  const std::string dp = std::to_string(pa_padded(c.q.D));
-  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H * a.parts, 1, 1, 256, s, a));
+  const std::string dp = std::to_string(a.DP);
+  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H * a.parts * (a.DP > 128 ? 2 : 1), 1, 1, 256, s, a));
   if (a.parts > 1) VH_TRY(launch("vh_pa_join_" + dp, a.max_tiles, c.k.H, 2, 256, s, a));
   return launch("vh_pa_dq_" + dp, a.max_blocks * c.q.H, 1, 1, 256, s, a);
 }

@@ -496,7 +496,7 @@ struct PaArgs {
   PaSpan* tiles;
   PaSpan* blocks;
   float* delta;            // [Hq][T]: sum over d of dout * out
-  int32_t n, T, D;
+  int32_t n, T, D, DP;     // DP: D padded to the kernels' size
   int32_t max_tiles, max_blocks, block_rows;
   int32_t causal;
   float scale;
