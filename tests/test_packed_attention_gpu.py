@@ -76,6 +76,18 @@ def test_many_short_sequences(vh):
     run_and_check(vh, lens, 2, 1, 32, True)
 
 
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_many_workgroups(vh, D):
+    """Enough blocks that dq and dk / dv go out as launches of their own."""
+    run_and_check(vh, [40] * 100, 8, 4, D, True, seed=D)
+
+
+@pytest.mark.parametrize("Hq,Hk,L", [(12, 4, 16), (16, 8, 32)])
+def test_parts_of_the_query_heads(vh, Hq, Hk, L):
+    """Enough key blocks that three query heads go to two workgroups unevenly, or two to one."""
+    run_and_check(vh, [L] * (16384 // L), Hq, Hk, 32, True, seed=L)
+
+
 def test_broadcast_keys(vh):
     """Every token and head reading one key row (zero strides): its gradient comes out per row."""
     lens, Hq, Hk, D = [40, 90], 4, 2, 64

@@ -221,3 +221,22 @@ def test_scratch_sizes():
     assert L.vh_linear_cross_entropy_scratch_bytes(1024, 8, 4000000, 1) >= 4 * 256 * 4000000
     assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 0) < 4 * 65536 * 50257 // 16
     assert L.vh_linear_cross_entropy_scratch_bytes(0, 8, 8, 1) == 0
+
+
+def test_code_object_holds_every_kernel():
+    import os
+
+    from conftest import ROOT
+    from test_abi_cpu import elf_symbols
+
+    path = os.path.join(ROOT, "vearo_amd", "csrc", "_build", "packed_kernels.co")
+    if not os.path.exists(path):
+        pytest.skip("code object not built in-tree")
+    names = {f"vh_rope_{d}_v{c}" for d in ("fwd", "bwd") for c in ("4_l4_n1", "4_l8_n1", "4_l16_n1", "4_l32_n1", "1_l64_n1",
+                                                                  "1_l64_n2")}
+    for dp in (32, 64, 96, 128, 192, 256):
+        names |= {f"vh_pa_{k}_{dp}" for k in ("prep", "fwd", "dq", "dkdv", "join")}
+    names |= {f"vh_pa_bwd_{dp}" for dp in (32, 64, 96, 128)}
+    names |= {"vh_lx_" + k for k in ("count", "stats", "grad", "stats_grad", "loss", "split", "logits", "finish")}
+    assert not names - elf_symbols(path)
+    assert open(path, "rb").read() in open(vh.LIB_PATH, "rb").read()

@@ -508,6 +508,10 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
 }
 
 // -------------------------------------------------------------------- backward --
+// LDS halves of the backward's workgroups: two stages of two tensors, and of the statistics.
+template <int DP>
+constexpr int kPaBwdLds = 4 * 64 * DP + 2 * 2 * 64;
+
 // dS under its running power of two 2^g: returns what to multiply dS by, 2^(g + sh)
 // where sh is the tile's difference from the accumulators' units, after lowering g (and
 // multiplying the accumulators over) where the tile's largest would pass 2^15.
@@ -535,10 +539,10 @@ VH_DEV float pa_fit(const pa_f16& ds, int sh, int& g, pa_f16 (&acc)[DB]) {
 // the forward, hold 32 registers more and a third stage of K: measured slower, 145 against
 // 125 us for 16384 tokens of 40 sequences, 12 heads of 64, at two waves a SIMD for three.)
 template <int DP, int NW>
-VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
+VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
   constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
-  const int H = a.q.H, id = blockIdx.x;
+  uint16_t(*lk)[SUB] = reinterpret_cast<uint16_t(*)[SUB]>(lds), (*lv)[SUB] = lk + 2;
+  const int H = a.q.H;
   const PaSpan sp = a.blocks[id / H];
   if (id >= a.head->nblocks * H) return;
   const int h = id % H, hk = h / (H / a.k.H);
@@ -625,11 +629,11 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a) {
 // whose sums pa_join adds in order. HALVES 2: a workgroup forms one half of dk's and dv's
 // elements, all of which are too many registers past 128.
 template <int DP, int NW, int HALVES>
-VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
+VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
   constexpr int KS = DP / 16, DB = DP / 32 / HALVES, SUB = 64 * DP;
-  __shared__ __attribute__((aligned(1024))) uint16_t lq[2][SUB], lg[2][SUB];
-  __shared__ __attribute__((aligned(1024))) float lst[2][64];  // a step's 32 log2-lse and 32 delta
-  const int H = a.k.H * a.parts, half = blockIdx.x % HALVES, id = blockIdx.x / HALVES;
+  uint16_t(*lq)[SUB] = reinterpret_cast<uint16_t(*)[SUB]>(lds), (*lg)[SUB] = lq + 2;
+  float(*lst)[64] = reinterpret_cast<float(*)[64]>(lds + 4 * SUB);  // a step's 32 log2-lse and 32 delta
+  const int H = a.k.H * a.parts, half = item % HALVES, id = item / HALVES;
   PaSpan sp = a.blocks[id / H];
   if (id >= a.head->nblocks * H) return;
   // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
@@ -744,6 +748,16 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a) {
   const int d0 = half * DB * 32, D = (whole ? a.D : DP) - d0;
   pa_store<DB>(to_k + d0, whole ? a.dk_vec : 1, D, dk, [&](float y) { return pa_ldexp(y * a.scale, topq - PA_E - PA_PV - g); });
   pa_store<DB>(to_v + d0, whole ? a.dv_vec : 1, D, dv, [&](float y) { return pa_ldexp(y, egc - PA_E - PA_PV); });
+}
+
+// Both in one launch, dk and dv first: where neither fills the chip, one runs beside the
+// other (256 tokens, 4 heads of 32: 20 -> 11.3 us). Where they do, dq alone has more waves a
+// SIMD.
+template <int DP, int NW>
+VH_DEV void pa_mm_bwd_impl(const PaArgs& a, uint16_t* lds) {
+  const int n = a.max_blocks * a.k.H * a.parts;
+  if ((int)blockIdx.x < n) pa_mm_dkdv_impl<DP, NW, 1>(a, blockIdx.x, lds);
+  else pa_mm_dq_impl<DP, NW>(a, blockIdx.x - n, lds);
 }
 
 // dk and dv of each token in a sequence: the parts' sums, in order. Grid: (tiles,

@@ -118,12 +118,16 @@ void rope_out(RopeArgs* a, float* yq, const vh_layout* qol, float* yk, const vh_
 int64_t pa_units(int64_t T, int64_t n, int64_t rows) { return T / rows + n; }
 
 constexpr int kPaBlockRows = 128;  // rows of a workgroup
+// dq with dk and dv in one launch up to this many workgroups of both: 256 tokens, 4 heads
+// of 32 37.6 -> 29.0 us for forward and backward, 4096 tokens, 12 heads of 64 (880
+// workgroups) 189 -> 163; one of 8192, 16 on 2 heads of 128 (2080) 3.90 -> 3.95 ms.
+constexpr int64_t kPaTogether = 1024;
 // The kernels' head sizes.
 int pa_padded(int64_t D) { return D <= 128 ? (int)cdiv(D, 32) * 32 : (int)cdiv(D, 64) * 64; }
 
 // Workgroups that share a key head's query heads in dk and dv: as many as bring the blocks
 // to kPaJoinBlocks, where a block's first keys meet every query after them. [8192] tokens, 16
-// query heads on 2 of 128: 128 workgroups take 7.2 ms for what 1024 do in PLACEHOLDER.
+// query heads on 2 of 128: 128 workgroups 7.2 ms, 1024 of an eighth each 2.2.
 constexpr int64_t kPaJoinBlocks = 1024;
 int pa_parts(int64_t T, int64_t Hq, int64_t Hk) {
   const int64_t G = Hq / Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk)));
@@ -501,9 +505,12 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   VH_TRY(pa_prepare(&c, lay, sc.p, true, s));
   const std::string dp = std::to_string(a.DP);
-  VH_TRY(launch("vh_pa_dkdv_" + dp, a.max_blocks * c.k.H * a.parts * (a.DP > 128 ? 2 : 1), 1, 1, 256, s, a));
+  const int64_t dkdv = a.max_blocks * c.k.H * a.parts * (a.DP > 128 ? 2 : 1), dqs = a.max_blocks * c.q.H;
+  // Few workgroups: both in one launch (pa_mm_bwd_impl).
+  const bool together = a.DP <= 128 && dkdv + dqs <= kPaTogether;
+  VH_TRY(launch((together ? "vh_pa_bwd_" : "vh_pa_dkdv_") + dp, together ? dkdv + dqs : dkdv, 1, 1, 256, s, a));
   if (a.parts > 1) VH_TRY(launch("vh_pa_join_" + dp, a.max_tiles, c.k.H, 2, 256, s, a));
-  return launch("vh_pa_dq_" + dp, a.max_blocks * c.q.H, 1, 1, 256, s, a);
+  return together ? VH_OK : launch("vh_pa_dq_" + dp, dqs, 1, 1, 256, s, a);
 }
 
 size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t D, int64_t V, int backward) {
