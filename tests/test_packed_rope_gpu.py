@@ -62,7 +62,7 @@ class Call:
 
 @pytest.mark.parametrize("inter", [0, 1])
 @pytest.mark.parametrize("D,rot", [(1, 0), (2, 2), (6, 4), (7, 6), (8, 8), (16, 8), (32, 32), (40, 40), (64, 64), (64, 32),
-                                   (64, 0), (65, 64), (80, 40), (96, 96), (100, 56), (127, 126), (128, 128), (128, 12),
+                                   (64, 0), (65, 64), (80, 40), (80, 80), (80, 16), (96, 96), (96, 24), (112, 112), (112, 42), (112, 0), (100, 56), (127, 126), (128, 128), (128, 12),
                                    (130, 130), (192, 64), (256, 256), (255, 130), (252, 248)])
 def test_head_sizes(vh, D, rot, inter):
     Call(vh, 37, 3, 2, D, rot, inter, seed=D).check()
@@ -77,7 +77,7 @@ def test_tokens_and_heads(vh, T, Hq, Hk):
 
 
 @pytest.mark.parametrize("kind", ["cols", "odd", "heads_first"])
-@pytest.mark.parametrize("D", [40, 64, 66])
+@pytest.mark.parametrize("D", [40, 64, 66, 80, 112])
 def test_layouts(vh, kind, D):
     Call(vh, 50, 4, 2, D, D // 4 * 2, 0, kind=kind).check()
 
