@@ -166,7 +166,8 @@ VH_DEV void lx_split_impl(const LxSplitArgs& a) {
 // formed in a lane. 16 elements a step, three LDS stages, two on their way.
 VH_DEV void lx_logits_impl(const LxLogitArgs& a) {
   constexpr int FW = VH_LX_TV / 32, FX = VH_LX_TR / 32, STAGE = (FW + FX) * 1024;  // halves
-  __shared__ __attribute__((aligned(1024))) uint16_t ls[3][STAGE];
+  __shared__ __attribute__((aligned(1024))) uint16_t stages[3 * STAGE];
+  const PaHalves ls = (PaHalves)stages;
   __shared__ float red[4][VH_LX_TR][2];
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5, li = lane & 31;
   // XCD x (the hardware deals workgroups out in turn) takes an eighth of the tiles, row
@@ -190,7 +191,7 @@ VH_DEV void lx_logits_impl(const LxLogitArgs& a) {
 #pragma unroll
     for (int k = 0; k < (FW + FX) / 4; ++k) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p) pa_copy16(from[k] + (int64_t)t * 1024 + p * 512, &ls[b][(w + 4 * k) * 1024 + p * 512]);
+      for (int p = 0; p < 2; ++p) pa_copy16(from[k] + (int64_t)t * 1024 + p * 512, ls + b * STAGE + (w + 4 * k) * 1024 + p * 512);
     }
   };
   pa_f16 acc[2][4];
@@ -206,9 +207,10 @@ VH_DEV void lx_logits_impl(const LxLogitArgs& a) {
     if (t + 1 < a.ke) pa_arrived_but<(FW + FX) / 2>();
     else pa_arrived();
     if (t + 2 < a.ke) stage(t + 2, b == 0 ? 2 : b - 1);
-    const uint16_t* p = ls[b] + (t & 1 ? row1 : row0);
+    const PaHalves p = ls + b * STAGE + (t & 1 ? row1 : row0);
     auto frag = [&](int f) {
-      return PaFrag{*reinterpret_cast<const pa_h8*>(p + f * 1024), *reinterpret_cast<const pa_h8*>(p + f * 1024 + 512)};
+      typedef const __attribute__((address_space(3))) pa_h8* Lds8;
+      return PaFrag{*(Lds8)(p + f * 1024), *(Lds8)(p + f * 1024 + 512)};
     };
     PaFrag fw[2], fx[4];
 #pragma unroll

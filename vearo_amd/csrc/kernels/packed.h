@@ -131,13 +131,14 @@ VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
 // cannot hold, about a hundred times slower: each lane reads a key's row by itself.
 
 // An LDS row of up to 256 elements that the wave alone reads and writes.
-VH_DEV void pa_row_to_lds(float* l, const float* p, int D) {
+typedef __attribute__((address_space(3))) float* PaLds;
+VH_DEV void pa_row_to_lds(PaLds l, const float* p, int D) {
   const int lane = threadIdx.x & 63;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   for (int d = lane; d < D; d += 64) l[d] = p[d];
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
-VH_DEV float pa_dot(const float* l, const float* p, int D) {
+VH_DEV float pa_dot(PaLds l, const float* p, int D) {
   float s = 0.0f;
   for (int d = 0; d < D; ++d) s = fmaf(l[d], p[d], s);
   return s;
@@ -156,7 +157,7 @@ VH_DEV void pa_axpy(float c, const float* x, int64_t st, int m, int D, float (&a
   }
 }
 
-VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, float* l) {
+VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l) {
   const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
   const int64_t tok = (int64_t)sp.start + i;
   const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
@@ -180,7 +181,7 @@ VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, float* l
   if (lane == 0) a.lse[(int64_t)h * a.T + tok] = m + logf(sum);
 }
 
-VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, float* l, float* lg) {
+VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l, PaLds lg) {
   const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
   const int64_t tok = (int64_t)sp.start + i;
   const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
@@ -204,7 +205,7 @@ VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, float* l,
 }
 
 // Over query heads h0 .. h1 - 1, into dk and dv or, of several parts, into this one's sums.
-VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float* l, float* lv, int h0, int h1, int part) {
+VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, PaLds l, PaLds lv, int h0, int h1, int part) {
   const int lane = threadIdx.x & 63;
   const int64_t tok = (int64_t)sp.start + j;
   pa_row_to_lds(l, a.k.p + tok * a.k.st + hk * a.k.sh, a.D);
@@ -241,13 +242,14 @@ VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, float*
 
 // The rows of one block, over the workgroup's waves. MODE 0 forward, 1 dq, 2 dk and dv.
 template <int MODE>
-VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, float (*l)[2][VH_PA_MAX_D], int h0 = 0, int h1 = 0,
+VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, PaLds l, int h0 = 0, int h1 = 0,
                     int part = 0) {
   const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int end = min(sp.len, sp.row0 + a.block_rows);
+  l += w * 2 * VH_PA_MAX_D;  // the wave's two rows
   for (int i = sp.row0 + w; i < end; i += nw) {
-    if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l[w][0]);
-    if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l[w][0], l[w][1]);
-    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l[w][0], l[w][1], h0, h1, part);
+    if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l);
+    if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l, l + VH_PA_MAX_D);
+    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l, l + VH_PA_MAX_D, h0, h1, part);
   }
 }

@@ -113,7 +113,7 @@ VH_DEV int pa_piece(int l, int k) { return l ^ (l >> 5 << 2) ^ ((k & 1) << 3); }
 // rows of each at a time, +inf and 0 past the sequence.
 template <int DP>
 VH_DEV void pa_prep_impl(const PaArgs& a) {
-  constexpr int KS = DP / 16, DB = DP / 32, LD = DP + 4;
+  constexpr int KS = DP / 16, LD = DP + 4;
   __shared__ __attribute__((aligned(16))) float x[64 * LD];
   __shared__ PaFind f;
   __shared__ uint32_t red[4][2];
@@ -140,7 +140,7 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
   float dl = 0.0f;
   const float* o = z == a.grad ? a.o.p + ((int64_t)sp.start + i) * a.o.st + h * a.o.sh : nullptr;
 #pragma unroll
-  for (int c = 0; c < DB * 2; ++c) {
+  for (int c = 0; c < KS; ++c) {
     const int d = 16 * c + 4 * (tid & 3);
     pa_f4 v = {0.0f, 0.0f, 0.0f, 0.0f}, u = v;
     if (live) {
@@ -212,20 +212,21 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
 }
 
 // ------------------------------------------------------------------ streaming --
+// LDS by its own address space: as generic pointers some of these kernels do not compile.
+typedef __attribute__((address_space(3))) uint16_t* PaHalves;
 // The wave's index in its workgroup, known to be the same for all its lanes.
 VH_DEV int pa_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 // 16 bytes a lane from memory to LDS byte `to` + 16 lane, past the registers. As inline
 // assembly (it has no output register) because after the builtin the compiler makes the
 // next LDS read, of whatever stage, wait for every such copy in flight. (m0, the copy's LDS
 // base, is a register that the compiler keeps nothing in.)
-VH_DEV void pa_copy16(const void* from, const void* to) {
-  const uint32_t l = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)to);
+VH_DEV void pa_copy16(const void* from, PaHalves to) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)to);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(from) : "memory");
 }
 // BYTES (a multiple of 1024) that way, waves taking 1024 in turn.
 template <int NW, int BYTES>
-VH_DEV void pa_copy(const uint16_t* from, const uint16_t* to) {
+VH_DEV void pa_copy(const uint16_t* from, PaHalves to) {
   const int lane = threadIdx.x & 63, w = pa_wave();
 #pragma unroll
   for (int u = 0; u < BYTES / 1024; u += NW)
@@ -252,30 +253,35 @@ VH_DEV PaInfo pa_info(const int32_t* p) { return (PaInfo)(uintptr_t)p; }
 // What a wave reads of a 32-token stage, 64 DP halves: [part][16 elements][piece].
 template <int DP>
 struct PaStage {
-  const uint16_t* base;
+  typedef const __attribute__((address_space(3))) uint16_t* Lds;
+  Lds base;
   int row, col;  // the lane's offset in a fragment by rows (k even), by columns (first four tokens)
-  VH_DEV PaStage(const uint16_t* b) : base(b) {
+  int last;      // col where the odd fragment of a pair is missing: the even one again, for
+                 // elements past DP
+  VH_DEV PaStage(Lds b) : base(b) {
     const int l = threadIdx.x & 63;
     row = pa_piece(l, 0) * 8;
     // The transposing read: lanes 4 k + c of 16 give token k's elements 4 c .. 4 c + 3
     // and lane i gets element i of the four tokens.
     const int i = l & 15, odd = l >> 4 & 1, k = i >> 2, c = i & 3;
     col = odd * 512 + pa_piece((c >> 1) * 32 + (l >> 5) * 4 + k, odd) * 8 + (c & 1) * 4;
+    last = col - odd * 512;
   }
   // Tokens by rows: elements 16 k .. 16 k + 15 of the 32 tokens.
   VH_DEV PaFrag rows(int st, int k) const {
-    const uint16_t* p = base + st * (64 * DP) + k * 512 + (k & 1 ? row ^ 64 : row);
-    return {*reinterpret_cast<const pa_h8*>(p), *reinterpret_cast<const pa_h8*>(p + DP / 16 * 512)};
+    typedef const __attribute__((address_space(3))) pa_h8* Lds8;
+    const Lds p = base + st * (64 * DP) + k * 512 + (k & 1 ? row ^ 64 : row);
+    return {*(Lds8)p, *(Lds8)(p + DP / 16 * 512)};
   }
   // Elements 32 db .. 32 db + 31 by rows, of 16 tokens: 8 (p / 4) + 4 (l / 32) + p % 4 past 16 u.
   VH_DEV PaFrag cols(int st, int db, int u) const {
-    const uint16_t* p = base + st * (64 * DP) + db * 1024 + u * 128;
-    auto four = [](const uint16_t* q) {
-      return __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                           (__attribute__((address_space(3))) pa_s4*)const_cast<uint16_t*>(q)));
+    const Lds p = base + st * (64 * DP) + db * 1024 + u * 128;
+    const int c = DP % 32 && db == DP / 32 ? last : col;
+    auto four = [](Lds q) {
+      return __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)q));
     };
-    auto eight = [&](const uint16_t* q) {
-      const pa_h4 a = four(q + col), b = four(q + (col ^ 64));
+    auto eight = [&](Lds q) {
+      const pa_h4 a = four(q + c), b = four(q + (c ^ 64));
       return pa_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     };
     return {eight(p), eight(p + DP / 16 * 512)};
@@ -395,8 +401,9 @@ VH_DEV void pa_scan(const PaStream& x, const PaStream& y, int H, int h, int t0, 
 // V's units at once: a branch around it costs the usual path more in copied registers.
 template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
-  constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  __shared__ __attribute__((aligned(1024))) uint16_t lk[2][SUB], lv[2][SUB];
+  constexpr int KS = DP / 16, DB = (DP + 31) / 32, SUB = 64 * DP;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * SUB];  // two stages of K, of V
+  const PaHalves lk = (PaHalves)lds, lv = lk + 2 * SUB;
   const int H = a.q.H, id = blockIdx.x;
   const PaSpan sp = a.blocks[id / H];  // (inside the table, also where it is not written)
   if (id >= a.head->nblocks * H) return;
@@ -404,15 +411,15 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
-  const PaStage<DP> fk(lk[0]), fv(lv[0]);
+  const PaStage<DP> fk(lk), fv(lv);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
   const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
-  auto stage = [&](const uint16_t* p, int t, uint16_t* to) {
+  auto stage = [&](const uint16_t* p, int t, PaHalves to) {
     pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
   };
-  stage(sk.n, 0, lk[0]);
-  stage(sv.n, 0, lv[0]);
-  if (nt > 1) stage(sk.n, 1, lk[1]);
+  stage(sk.n, 0, lk);
+  stage(sv.n, 0, lv);
+  if (nt > 1) stage(sk.n, 1, lk + SUB);
   PaFrag q[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q);
   PaRange rk, rv;
@@ -421,7 +428,7 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   int top;
   if (rv.any_slow(top)) {
     pa_arrived();  // (nothing on its way into the rows' LDS)
-    pa_rows<0>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
+    pa_rows<0>(a, h, sp, (PaLds)lk);
     return;
   }
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
@@ -439,8 +446,8 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   // Step t's V and step t + 1's K are in LDS; V of t + 1 and K of t + 2 go out.
   auto arrive = [&](int t) {
     if (t) pa_arrived();
-    if (t + 1 < nt) stage(sv.n, t + 1, lv[(t + 1) & 1]);
-    if (t + 2 < nt) stage(sk.n, t + 2, lk[t & 1]);
+    if (t + 1 < nt) stage(sv.n, t + 1, lv + ((t + 1) & 1) * SUB);
+    if (t + 2 < nt) stage(sk.n, t + 2, lk + (t & 1) * SUB);
   };
   auto step = [&](int t, auto last) {
     const int b = t & 1, ek = ekn, evt = evn;
@@ -539,9 +546,9 @@ VH_DEV float pa_fit(const pa_f16& ds, int sh, int& g, pa_f16 (&acc)[DB]) {
 // the forward, hold 32 registers more and a third stage of K: measured slower, 145 against
 // 125 us for 16384 tokens of 40 sequences, 12 heads of 64, at two waves a SIMD for three.)
 template <int DP, int NW>
-VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
-  constexpr int KS = DP / 16, DB = DP / 32, SUB = 64 * DP;
-  uint16_t(*lk)[SUB] = reinterpret_cast<uint16_t(*)[SUB]>(lds), (*lv)[SUB] = lk + 2;
+VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, PaHalves lds) {
+  constexpr int KS = DP / 16, DB = (DP + 31) / 32, SUB = 64 * DP;
+  const PaHalves lk = lds, lv = lds + 2 * SUB;
   const int H = a.q.H;
   const PaSpan sp = a.blocks[id / H];
   if (id >= a.head->nblocks * H) return;
@@ -549,15 +556,15 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
-  const PaStage<DP> fk(lk[0]), fv(lv[0]);
+  const PaStage<DP> fk(lk), fv(lv);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
   const bool live = i < sp.len;
   const int64_t base = ((int64_t)sp.tile0 * a.k.H + hk) * (2 * SUB), chunk = (int64_t)a.k.H * (2 * SUB);
-  auto stage = [&](const uint16_t* p, int t, uint16_t* to) {
+  auto stage = [&](const uint16_t* p, int t, PaHalves to) {
     pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
   };
-  stage(sk.n, 0, lk[0]);
-  stage(sv.n, 0, lv[0]);
+  stage(sk.n, 0, lk);
+  stage(sv.n, 0, lv);
   PaFrag q[KS], gq[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q), eg = pa_own<DP>(a.g, sp, a.D, i, h, gq);
   PaRange rk, rv;
@@ -566,7 +573,7 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
   int top;
   if (rk.any_slow(top)) {
     pa_arrived();
-    pa_rows<1>(a, h, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lk[0][0]));
+    pa_rows<1>(a, h, sp, (PaLds)lk);
     return;
   }
   const int64_t tok = (int64_t)sp.start + i;
@@ -585,8 +592,8 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
     pa_arrived();
     const int b = t & 1, ek = ekn, ev = evn;
     if (t + 1 < nt) {
-      stage(sk.n, t + 1, lk[b ^ 1]);
-      stage(sv.n, t + 1, lv[b ^ 1]);
+      stage(sk.n, t + 1, lk + (b ^ 1) * SUB);
+      stage(sv.n, t + 1, lv + (b ^ 1) * SUB);
       const int64_t ahead = (int64_t)((t + 1) >> 1) * a.k.H;
       ekn = ik[ahead];
       evn = iv[ahead];
@@ -629,10 +636,9 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, uint16_t* lds) {
 // whose sums pa_join adds in order. HALVES 2: a workgroup forms one half of dk's and dv's
 // elements, all of which are too many registers past 128.
 template <int DP, int NW, int HALVES>
-VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
-  constexpr int KS = DP / 16, DB = DP / 32 / HALVES, SUB = 64 * DP;
-  uint16_t(*lq)[SUB] = reinterpret_cast<uint16_t(*)[SUB]>(lds), (*lg)[SUB] = lq + 2;
-  float(*lst)[64] = reinterpret_cast<float(*)[64]>(lds + 4 * SUB);  // a step's 32 log2-lse and 32 delta
+VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, PaHalves lds) {
+  constexpr int KS = DP / 16, DB = (DP + 31) / 32 / HALVES, SUB = 64 * DP;
+  const PaHalves lq = lds, lg = lds + 2 * SUB, lst = lds + 4 * SUB;  // lst: a step's 32 log2-lse and 32 delta
   const int H = a.k.H * a.parts, half = item % HALVES, id = item / HALVES;
   PaSpan sp = a.blocks[id / H];
   if (id >= a.head->nblocks * H) return;
@@ -644,8 +650,9 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1], &sq = a.stream[2], &sg = a.stream[3];
   const int t0 = a.causal ? sp.row0 >> 5 : 0, t1 = (sp.len + 31) >> 5;
-  const PaStage<DP> fq(lq[0]), fg(lg[0]);
+  const PaStage<DP> fq(lq), fg(lg);
   const int r0 = sp.row0 + 32 * w, j = r0 + (lane & 31);
+  auto stat = [&](int b, int i) { return *(const __attribute__((address_space(3))) pa_f4*)(lst + b * 128 + 2 * i); };
   const int nt = t1 - t0, steps = nt * (h1 - h0);
   struct At {  // a step's head and 32 queries
     int h, t;
@@ -659,9 +666,9 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
   auto tile = [&](At x) { return (int64_t)(sp.tile0 + (x.t >> 1)) * a.q.H + x.h; };
   auto stage = [&](At x, int st) {
     const int64_t at = tile(x) * (2 * SUB) + (x.t & 1) * SUB;
-    pa_copy<NW, 2 * SUB>(sq.n + at, lq[st]);
-    pa_copy<NW, 2 * SUB>(sg.n + at, lg[st]);
-    if (threadIdx.x < 16) pa_copy16(a.stat + tile(x) * 128 + (x.t & 1) * 64 + threadIdx.x * 4, lst[st]);
+    pa_copy<NW, 2 * SUB>(sq.n + at, lq + st * SUB);
+    pa_copy<NW, 2 * SUB>(sg.n + at, lg + st * SUB);
+    if (threadIdx.x < 16) pa_copy16(a.stat + tile(x) * 128 + (x.t & 1) * 64 + threadIdx.x * 4, lst + st * 128);
   };
   At now{h0, t0}, ahead{h0, t0};  // ahead: the last step staged
   if (steps > 0) stage(ahead, 0);
@@ -676,7 +683,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
   const bool slow_q = rq.any_slow(topq), slow_g = rg.any_slow(topg);
   if (slow_q || slow_g) {
     pa_arrived();
-    if (half == 0) pa_rows<2>(a, hk, sp, reinterpret_cast<float(*)[2][VH_PA_MAX_D]>(&lq[0][0]), h0, h1, part);
+    if (half == 0) pa_rows<2>(a, hk, sp, (PaLds)lq, h0, h1, part);
     return;
   }
   const float cs = a.scale * PA_LOG2E;
@@ -716,7 +723,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
     // Register r is query 32 t + 8 (r / 4) + 4 hf + r % 4, the lane's column key j.
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const pa_f4 ls4 = *reinterpret_cast<const pa_f4*>(&lst[b][8 * y + 4 * hf]);
+      const pa_f4 ls4 = stat(b, 8 * y + 4 * hf);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * y + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + e], c, -ls4[e]));
     }
@@ -728,7 +735,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const pa_f4 dl4 = *reinterpret_cast<const pa_f4*>(&lst[b][32 + 8 * y + 4 * hf]);
+      const pa_f4 dl4 = stat(b, 32 + 8 * y + 4 * hf);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * y + e] *= fmaf(dp[4 * y + e], cg, -dl4[e]);
     }
@@ -754,7 +761,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, uint16_t* lds) {
 // other (256 tokens, 4 heads of 32: 20 -> 11.3 us). Where they do, dq alone has more waves a
 // SIMD.
 template <int DP, int NW>
-VH_DEV void pa_mm_bwd_impl(const PaArgs& a, uint16_t* lds) {
+VH_DEV void pa_mm_bwd_impl(const PaArgs& a, PaHalves lds) {
   const int n = a.max_blocks * a.k.H * a.parts;
   if ((int)blockIdx.x < n) pa_mm_dkdv_impl<DP, NW, 1>(a, blockIdx.x, lds);
   else pa_mm_dq_impl<DP, NW>(a, blockIdx.x - n, lds);

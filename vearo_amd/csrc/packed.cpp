@@ -123,7 +123,7 @@ constexpr int kPaBlockRows = 128;  // rows of a workgroup
 // workgroups) 189 -> 163; one of 8192, 16 on 2 heads of 128 (2080) 3.90 -> 3.95 ms.
 constexpr int64_t kPaTogether = 1024;
 // The kernels' head sizes.
-int pa_padded(int64_t D) { return D <= 128 ? (int)cdiv(D, 32) * 32 : (int)cdiv(D, 64) * 64; }
+int pa_padded(int64_t D) { return D <= 32 ? 32 : D <= 128 ? (int)cdiv(D, 16) * 16 : (int)cdiv(D, 64) * 64; }
 
 // Workgroups that share a key head's query heads in dk and dv: as many as bring the blocks
 // to kPaJoinBlocks, where a block's first keys meet every query after them. [8192] tokens, 16
