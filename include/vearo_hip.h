@@ -452,7 +452,8 @@ int vh_qk_norm_rope_fwd(const float* q, const vh_layout* ql, const float* k, con
                         void* stream);
 /* Its backward from the same inputs and the results' gradients dqo, dko: dq, dk, and the
  * weights' gradients dwq[D], dwk[D], summed over tokens and heads in a fixed order (no
- * atomics). dq may be dqo or q, and dk dko or k, in the same layout. scratch: NULL or
+ * atomics): over all T tokens, so tokens in no sequence need finite rows and zeros in dqo
+ * and dko. dq may be dqo or q, and dk dko or k, in the same layout. scratch: NULL or
  * vh_qk_norm_rope_bwd_scratch_bytes(T, D) bytes. */
 int vh_qk_norm_rope_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* wq,
                         const float* wk, const float* positions, float eps, double base, int32_t rotary,
@@ -463,11 +464,13 @@ size_t vh_qk_norm_rope_bwd_scratch_bytes(int64_t T, int64_t D);
 
 /* Attention within each of n packed sequences, with grouped heads: q, out: [T, Hq, D];
  * k, v: [T, Hk, D]; query head h reads key head h / (Hq / Hk); Hq a multiple of Hk,
- * D <= 256. starts: n + 1 int32 in device memory, not decreasing, in [0, T]: sequence s
+ * D <= 256, T <= 2^28. starts: n + 1 int32 in device memory, not decreasing, in [0, T]: sequence s
  * is tokens starts[s] .. starts[s + 1] - 1 (it may be empty); tokens in no sequence are
  * not read, and their rows of every output are left as they were. With causal != 0 a
  * query sees the keys up to its own token, else its whole sequence; what a query does not
- * see does not reach its row, infinities and NaN included. scale > 0 multiplies the
+ * see does not reach its row, infinities and NaN included. Blocks of 128 rows that meet
+ * infinities, NaN, or neighbouring rows 2^20 (k, v) or 2^30 (q, dout) apart are computed
+ * row by row, right but about a hundred times slower. scale > 0 multiplies the
  * scores. lse: [Hq, T], each row's log of the sum of exp of its scores, kept for the
  * backward. Scores are never stored. A starts array that breaks its rule computes nothing
  * and raises VH_ERR_DEVICE_PANIC at the next vh_sync.
@@ -488,13 +491,14 @@ size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64
 /* loss[0] = mean over the counted rows r of -log_softmax(x[r] w^T)[targets[r]], without
  * keeping the [R, V] logits: a forward alone reduces them as they are formed, a gradient
  * forms them in pieces of rows, in scratch (at most 1 GiB of logits, 256 rows at least).
- * An infinity in x or w counts as NaN. x: R rows of D,
- * ldx floats apart; w: V rows of D, ldw apart; targets: [R] f32 class ids as above, a row
- * whose target equals `ignore` not counted (NaN: none is). No counted row: loss 0.
+ * An infinity in x or w counts as NaN. x: R rows of D, ldx floats apart; w: V rows of D,
+ * ldw apart; targets: [R] f32 class ids as above, a row whose target equals `ignore` not
+ * counted (NaN: none is): its dx is zero and nothing of it reaches dw, NaN included. No
+ * counted row: loss 0.
  * row_stats: [R, 2], each row's max logit and sum of exp(logit - max), kept for the
  * backward (8-byte aligned). scratch: NULL or
- * vh_linear_cross_entropy_scratch_bytes(R, D, V, 0) bytes (1 with a gradient). Not under graph capture
- * (VH_ERR_UNSUPPORTED: the products inside take workspaces of their own). */
+ * vh_linear_cross_entropy_scratch_bytes(R, D, V, 0) bytes (1 with a gradient). Not under
+ * graph capture (VH_ERR_UNSUPPORTED: the products inside take workspaces of their own). */
 int vh_linear_cross_entropy_fwd(const float* x, int64_t ldx, const float* w, int64_t ldw, const float* targets,
                                 float ignore, float* loss, float* row_stats, int64_t R, int64_t D, int64_t V,
                                 void* scratch, size_t scratch_bytes, void* stream);

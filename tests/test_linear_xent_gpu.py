@@ -153,6 +153,36 @@ def test_bad_values_stay_in_their_row(vh, sizes):
     np.testing.assert_array_equal(got["stats"][keep], clean["stats"][keep])
 
 
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
+def test_ignored_rows_reach_nothing(vh, sizes, bad):
+    """What a row that is not counted holds reaches neither the loss nor dw, and its dx is zero."""
+    c = Xent(vh, *sizes, 0.3)
+    c.t[-1] = -100
+    off = c.t == -100
+    val, tol = R.linear_xent(c.x, c.w, c.t, c.ignore, c.go)
+    c.x[off] = bad
+    for calls in (("fwd", "bwd"), ("fwd_bwd",)):
+        c.put()
+        for which in calls:
+            c.call(which)
+        got = c.results()
+        assert not got["dx"][off].any()
+        R.check(got, val, tol, ["loss", "dx", "dw"])
+
+
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+@pytest.mark.parametrize("power", [-100, 100])
+def test_large_weights_of_small_rows(vh, sizes, power):
+    """Logits of a usual size whose factors are far from one."""
+    c = Xent(vh, *sizes, 0.1)
+    c.x = np.ldexp(c.x, power).astype(np.float32)
+    c.w = np.ldexp(c.w, -power).astype(np.float32)
+    c.put()
+    c.call("fwd")
+    R.check(c.results(), *R.linear_xent(c.x, c.w, c.t, c.ignore, c.go), ["loss", "stats"])
+
+
 def test_same_bits_and_streams(vh):
     c = Xent(vh, 700, 64, 3001, 0.1)
     c.call("fwd_bwd")

@@ -191,6 +191,18 @@ def test_rows_of_very_different_size(vh, name, spread, causal):
     run_and_check(vh, lens, 2, 1, D, causal, arrays=tuple(a.values()))
 
 
+@pytest.mark.parametrize("lens,Hq,Hk,D", [([700], 8, 1, 32), ([300], 6, 2, 64), ([40] * 100, 8, 4, 128), ([150], 4, 1, 160),
+                                          ([200], 2, 1, 256)])
+def test_rows_of_very_different_size_in_every_launch(vh, lens, Hq, Hk, D):
+    """The row forms beside the matrix kernels: query heads in parts, dq with dk and dv, each alone, elements in halves."""
+    for n in range(4):
+        a = list(inputs(lens, Hq, Hk, D, 21))
+        rows = np.ones(sum(lens), np.float32)
+        rows[5:60:7] = 1e-11
+        a[n] = (a[n] * rows[:, None, None]).astype(np.float32)
+        run_and_check(vh, lens, Hq, Hk, D, True, arrays=tuple(a))
+
+
 def test_rising_tiles(vh):
     """Values that grow or shrink a thousandfold from tile to tile (running scales)."""
     lens, D = [400], 64
@@ -245,7 +257,7 @@ def test_gradients_against_differences(vh):
 
 @pytest.mark.parametrize("starts,at,value", [([0, 40, 30, 100], 2, 30), ([0, 50, 101], 2, 101), ([-1, 50, 100], 0, -1),
                                              ([0, 2 ** 31 - 1, 100], 1, 2 ** 31 - 1), ([120, 130], 0, 120),
-                                             ([0, -5, 100], 1, -5)])
+                                             ([0, -5, 100], 1, -5), ([0, 100] * 300, 2, 0)])
 @pytest.mark.parametrize("D", [64, 160])
 def test_bad_starts(vh, starts, at, value, D):
     a = inputs([100], 2, 1, D)

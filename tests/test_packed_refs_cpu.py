@@ -155,11 +155,14 @@ def attention_bwd_args(**kw):
     (vh.VH_ERR_INVALID, "scale", {"scale": math.inf}),
     (vh.VH_ERR_INVALID, "multiple", {"kl": lay(4, 3, 8), "vl": lay(4, 3, 8)}),
     (vh.VH_ERR_INVALID, "multiple", {"kl": lay(4, 0, 8), "vl": lay(4, 0, 8)}),
+    (vh.VH_ERR_INVALID, "multiple", {"ql": lay(4, 0, 8), "ol": lay(4, 0, 8)}),
     (vh.VH_ERR_INVALID, "shape", {"vl": lay(4, 1, 8)}), (vh.VH_ERR_INVALID, "shape", {"ol": lay(4, 4, 6)}),
     (vh.VH_ERR_INVALID, "null", {"starts": None}), (vh.VH_ERR_INVALID, "null", {"lse": None}),
     (vh.VH_ERR_INVALID, "null", {"v": None}), (vh.VH_ERR_INVALID, "null", {"o": None}),
     (vh.VH_ERR_UNSUPPORTED, "unit stride", {"kl": lay(4, 2, 8, strides=[16, 1, 2])}),
     (vh.VH_ERR_UNSUPPORTED, "range", {"n": 2 ** 31}),
+    (vh.VH_ERR_UNSUPPORTED, "range", {"ql": lay(2 ** 28 + 1, 4, 8), "ol": lay(2 ** 28 + 1, 4, 8),
+                                      "kl": lay(2 ** 28 + 1, 2, 8), "vl": lay(2 ** 28 + 1, 2, 8)}),
 ])
 def test_attention_refusals(code, text, kw):
     refused(code, text, "vh_packed_attention_fwd", *attention_args(**kw))

@@ -74,6 +74,9 @@ VH_DEV void pa_find(const PaArgs& a, int idx, PaFind& f, int (&tot)[2]) {
       tot[0] += f.wave[k][0];
       tot[1] += f.wave[k][1];
     }
+    // No tables have as many (T <= VH_PA_MAX_T): starts that go back and forth would pass int.
+    tot[0] = min(tot[0], 2 * VH_PA_MAX_T);
+    tot[1] = min(tot[1], 2 * VH_PA_MAX_T);
     __syncthreads();
     if (!ALL && tot[0] > idx && tot[1] > idx) break;
   }
@@ -118,12 +121,12 @@ VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
   if (threadIdx.x == 0 && f.tile.len >= 0 && idx < a.max_tiles) a.tiles[idx] = f.tile;
   if (f.block.len >= 0 && idx < a.max_blocks) {
     const int at = pa_rank(a, f.block, f);
-    // (Starts out of order could rank two blocks alike: then none is used.)
-    if (threadIdx.x == 0 && at < a.max_blocks) a.blocks[at] = f.block;
+    // (Starts out of order could rank two blocks alike, or past int: then none is used.)
+    if (threadIdx.x == 0 && (uint32_t)at < (uint32_t)a.max_blocks) a.blocks[at] = f.block;
   }
 }
 
-// ------------------------------------------------------------ row kernels --
+// -------------------------------------------------------------- row forms --
 // A wave per row, keys over its lanes for the scores, elements over its lanes for
 // the products. Scores are formed again in each pass instead of kept, so a row may
 // have any length. f32 arithmetic throughout, element by element, nothing masked

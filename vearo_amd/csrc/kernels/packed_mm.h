@@ -1,13 +1,16 @@
-// packed_mm.h -- attention over packed sequences on the f16 matrix instruction: f32 products carried by two f16 parts per operand.
+// packed_mm.h -- attention over packed sequences on the f16 matrix instruction: f32
+// products carried by two f16 parts per operand.
 //
 // An f32 value scaled to |x| < 2^15 is h + l + r, h = f16(x), l = f16(x - h), with
 // |r| <= 2^-22 |x| down to 2^-18 of the largest value the scale was made for and
 // 2^-40 of that value below. Three products then carry an f32 one,
 //   x y = h h' + h l' + l h' + [l l' + r y + x r'],
-// the bracket being below 3 * 2^-22 |x y| and random in sign: what the softmax does
-// to a rounding of its scores is larger (exp of a score of 8 makes 2^-21 of half an
-// ulp). Against three bf16 parts (split3.h) that is half the matrix instructions; f16's
-// short exponent is paid for with scales:
+// the bracket being below 3 * 2^-22 |x y| and random in sign. The softmax does no
+// less to f32's own roundings (a score of 8 that is off by its last place's half,
+// 2^-22, moves its exp by 2^-22 of it), so the results are as far from 64 bits as plain
+// f32 attention's: 1.5e-7 against 2.9e-7 of the norm and below (the cases' table). Against
+// three bf16 parts (split3.h) that is half the matrix instructions; f16's short exponent
+// is paid for with scales:
 //   - a tensor that is streamed (K and V by the forward and dq, Q and dO by dk/dv) has
 //     one power of two per tile of 64 tokens and head, from the tile's largest value;
 //   - one that a wave holds has one per row, which is a lane there;
@@ -15,10 +18,17 @@
 //     is lowered when a tile's largest needs it, as the softmax's running maximum is.
 // A sum over tiles is in the units of one of them: what a tile's power of two differs by
 // goes into the other operand (into dS's own scale; into P's while it is within
-// PA_SHIFT, beyond which the accumulators are multiplied over, exactly). A tile whose rows differ by more than VH_PA_SPAN_KV (K, V) or
-// VH_VH_PA_SPAN_Q (Q, dO) powers of two, tiles of one stream that differ by more than
-// PA_SPAN_TILES, and infinities and NaN send the workgroup's block to the row kernels of
-// packed.h, which have no such limits.
+// PA_SHIFT, beyond which the accumulators are multiplied over, exactly). A tile whose rows
+// differ by more than VH_PA_SPAN_KV (K, V) or VH_PA_SPAN_Q (Q, dO) powers of two, tiles of
+// one stream that differ by more than PA_SPAN_TILES, and infinities and NaN send the
+// workgroup's block to the row forms of packed.h, which have no such limits. (20 keeps a
+// small row's error in a tile below 2^-20 of that row also where the large one is not seen;
+// the rows of Q and dO meet only in sums where the large one outweighs it.)
+//
+// What bounds it: the chip's power, as a large f16 library product (1090 TFLOP/s here; a
+// third is 363 of f32 products). One sequence of 8192, 16 on 2 heads of 128: forward 0.76
+// ms, 1090 TFLOP/s of f16; dq 1.17, 1060; dk and dv 1.73, 970. 16 of 1024, 12 on 4 heads
+// of 64: forward 95 us, 850, vector and matrix work in the same order of cycles.
 //
 // A first launch (pa_prep) splits the streamed tensors once, into the order the
 // matrix instruction's lanes take them: a fragment is 32 tokens x 16 elements of one part,
@@ -107,10 +117,10 @@ VH_DEV float pa_sum_halves(float v) {
 VH_DEV int pa_piece(int l, int k) { return l ^ (l >> 5 << 2) ^ ((k & 1) << 3); }
 
 // ------------------------------------------------------------------- prepare --
-// Grid: (tiles or blocks, whichever more; heads; tensors). The tensor's tile goes through
-// LDS once and out as fragments. The gradient's workgroups also
-// write delta and, per tile, what dk/dv reads per query: log2-lse - PA_PV and delta, 32
-// rows of each at a time, +inf and 0 past the sequence.
+// Grid: (tiles, heads, tensors). The tensor's tile goes through LDS once and out as
+// fragments. The gradient's workgroups also write delta and, per tile, what dk/dv reads
+// per query: log2-lse - PA_PV and delta, 32 rows of each at a time, +inf and 0 past the
+// sequence. Memory bound: 4.4 TB/s of the copy's 5.0 over [16384, 12, 64] x 2.
 template <int DP>
 VH_DEV void pa_prep_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, LD = DP + 4;
@@ -161,9 +171,8 @@ VH_DEV void pa_prep_impl(const PaArgs& a) {
   }
   // The row's largest over its four threads, then the tile's largest and smallest (of
   // rows that are not zero).
-  auto quad = [](uint32_t v, int ctrl) { return ctrl == 1 ? __builtin_amdgcn_update_dpp(0, (int)v, DPP_QUAD_XOR1, 0xF, 0xF, false) : __builtin_amdgcn_update_dpp(0, (int)v, DPP_QUAD_XOR2, 0xF, 0xF, false); };
-  big = max(big, (uint32_t)quad(big, 1));
-  big = max(big, (uint32_t)quad(big, 2));
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, DPP_QUAD_XOR1, 0xF, 0xF, false));
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, DPP_QUAD_XOR2, 0xF, 0xF, false));
   if (z == a.grad) {
     dl = group_sum<4>(dl);
     const int64_t tok = (int64_t)h * a.T + sp.start + i;
@@ -395,10 +404,12 @@ VH_DEV void pa_scan(const PaStream& x, const PaStream& y, int H, int h, int t0, 
 // -------------------------------------------------------------------- forward --
 // A workgroup per block of 32 NW queries and head, 32 queries a wave; keys in steps of
 // 32 through two LDS stages. A step multiplies the next step's S while its own P is formed
-// and multiplied by V: the matrix unit and the vector unit (exp is a quarter rate) have
-// about as much to do, and a wave alone would have them take turns. So K runs one step
+// and multiplied by V: the matrix unit and the vector unit have about as much
+// to do, and a wave alone would have them take turns. So K runs one step
 // ahead of V. The accumulators are multiplied over at every step, to the new maximum and to
-// V's units at once: a branch around it costs the usual path more in copied registers.
+// V's units at once: a branch around it costs the usual path more in copied registers
+// (16 x 1024 tokens, 12 on 4 heads of 64: 106 us with it at three waves a SIMD, 95 without
+// at four). Workgroups of 64 queries instead of 128: 126.
 template <int DP, int NW>
 VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   constexpr int KS = DP / 16, DB = (DP + 31) / 32, SUB = 64 * DP;

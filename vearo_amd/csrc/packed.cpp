@@ -183,9 +183,9 @@ int pa_check(const std::string& f, const float* q, const vh_layout* ql, const fl
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(VH_ERR_INVALID, f + ": scale must be positive and finite");
   if (D < 1 || D > VH_PA_MAX_D)
     return fail(VH_ERR_UNSUPPORTED, f + ": head size must be in [1, " + std::to_string(VH_PA_MAX_D) + "]");
-  if (c->k.H == 0 ? c->q.H != 0 : c->q.H % c->k.H != 0)
-    return fail(VH_ERR_INVALID, f + ": query heads must be a multiple of key heads");
-  if (T > INT32_MAX - 256 || n > INT32_MAX / 2 || c->q.H > 65535)
+  if (c->k.H == 0 ? c->q.H != 0 : c->q.H == 0 || c->q.H % c->k.H != 0)
+    return fail(VH_ERR_INVALID, f + ": query heads must be a positive multiple of key heads");
+  if (T > VH_PA_MAX_T || n > INT32_MAX / 2 || c->q.H > 65535)
     return fail(VH_ERR_UNSUPPORTED, f + ": size outside the implemented range");
   c->empty = T == 0 || n == 0 || c->q.H == 0;
   if (c->empty) return VH_OK;
@@ -248,7 +248,7 @@ int64_t lx_rows(int64_t R, int64_t D, int64_t V, bool backward) {
   return std::min<int64_t>(R, cdiv(cdiv(R, cdiv(R, fit)), 256) * 256);
 }
 struct LxScratch {
-  size_t z, row_loss, inv, stats, xf, xe, wf, we, part, zt, total;
+  size_t z, xs, row_loss, inv, stats, xf, xe, wf, we, part, zt, total;
   LxScratch(int64_t R, int64_t D, int64_t V, bool backward) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -259,6 +259,7 @@ struct LxScratch {
     const bool parts = lx_by_parts(R, D, V);
     const int64_t rows = lx_rows(R, D, V, backward);
     z = take(parts && !backward ? 0 : sizeof(float) * (size_t)(rows * lx_ld(V)));
+    xs = take(backward ? sizeof(float) * (size_t)(rows * lx_ld(D)) : 0);
     row_loss = take(sizeof(float) * (size_t)R);
     inv = take(256);
     stats = take(backward ? 2 * sizeof(float) * (size_t)R : 0);  // (of a call that returns none)
@@ -329,7 +330,7 @@ int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes,
   auto exps = [&](size_t off) { return reinterpret_cast<int32_t*>(base + off); };
   float *z = at(lay.z), *row_loss = at(lay.row_loss), *inv = at(lay.inv);
   float* stats = c.stats ? c.stats : at(lay.stats);
-  const int64_t ld = lx_ld(c.V), piece = lx_rows(c.R, c.D, c.V, c.backward);
+  const int64_t ld = lx_ld(c.V), ldxs = lx_ld(c.D), piece = lx_rows(c.R, c.D, c.V, c.backward);
   const bool parts = lx_by_parts(c.R, c.D, c.V);
   const int32_t V = (int32_t)c.V, ke = (int32_t)(cdiv(c.D, 32) * 2);
   auto split = [&](const float* p, int64_t stride, int64_t rows, size_t f, size_t e) {
@@ -357,10 +358,12 @@ int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes,
     }
     const char* kernel = parts || !c.forward ? "vh_lx_grad" : c.backward ? "vh_lx_stats_grad" : "vh_lx_stats";
     if (c.backward || !parts)
-      VH_TRY(launch(kernel, rows, 1, 1, 512, s, LxArgs{z, t, c.grad_out, inv, st, row_loss + r, rows, ld, V, c.ignore}));
+      VH_TRY(launch(kernel, rows, 1, 1, 512, s, 
+                    LxArgs{z, t, c.grad_out, inv, st, row_loss + r, x, at(lay.xs), rows, ld, c.ldx, ldxs, V, (int32_t)c.D,
+                           c.ignore}));
     if (!c.backward) continue;
     VH_TRY(lx_product(rows, c.D, c.V, z, ld, 1, c.w, c.ldw, 1, c.dx + r * c.lddx, c.lddx, false, s));
-    VH_TRY(lx_product(c.V, c.D, rows, z, 1, ld, x, c.ldx, 1, c.dw, c.lddw, r > 0, s));
+    VH_TRY(lx_product(c.V, c.D, rows, z, 1, ld, at(lay.xs), ldxs, 1, c.dw, c.lddw, r > 0, s));
   }
   if (c.forward) VH_TRY(launch("vh_lx_loss", 1, 1, 1, 1024, s, LxLossArgs{row_loss, inv, c.loss, c.R}));
   return VH_OK;

@@ -450,6 +450,7 @@ struct RopeArgs {
 
 // Attention over packed sequences (kernels/packed.h).
 #define VH_PA_MAX_D 256
+#define VH_PA_MAX_T (1 << 28)  // packed tokens
 #define VH_PA_SPAN_KV 20  // powers of two that rows of a tile of K or V, of Q or dO may
 #define VH_PA_SPAN_Q 30   // differ by on the matrix kernels
 // Workspace header, then the tables. A tile is 64 tokens of one sequence, a block
@@ -512,8 +513,10 @@ struct LxArgs {
   const float* inv;      // 1 / counted rows (0 if there is none)
   float* stats;          // of the piece: [rows][2] row max, sum of exp
   float* row_loss;       // of the piece, or null
-  int64_t rows, ld;
-  int32_t V;
+  const float* x;        // of the piece, and
+  float* xs;             // its copy, rows that are not counted as zeros (GRAD)
+  int64_t rows, ld, ldx, ldxs;
+  int32_t V, D;
   float ignore;
 };
 struct LxCountArgs {
