@@ -490,7 +490,8 @@ size_t vh_packed_attention_scratch_bytes(int64_t T, int64_t n, int64_t Hq, int64
 
 /* loss[0] = mean over the counted rows r of -log_softmax(x[r] w^T)[targets[r]], without
  * keeping the [R, V] logits: a forward alone reduces them as they are formed, a gradient
- * forms them in pieces of rows, in scratch (at most 1 GiB of logits, 256 rows at least).
+ * forms them in pieces of rows, in scratch (683 MiB of logits at most, 256 rows at least,
+ * and where the sizes are large three times that, and a copy of w).
  * An infinity in x or w counts as NaN. x: R rows of D, ldx floats apart; w: V rows of D,
  * ldw apart; targets: [R] f32 class ids as above, a row whose target equals `ignore` not
  * counted (NaN: none is): its dx is zero and nothing of it reaches dw, NaN included. No

@@ -12,6 +12,7 @@ from test_packed_rope_gpu import Call
 from test_streams_gpu import Streams
 
 pytestmark = pytest.mark.gpu
+BIG = (1100, 700, 17003)  # the gradient's products by f16 parts too
 
 
 class Xent:
@@ -84,8 +85,15 @@ def test_strided_rows(vh, pad, offset):
     Xent(vh, 130, 60, 700, 0.2, pad=pad, offset=offset).check()
 
 
+@pytest.mark.parametrize("sizes,pad", [((1025, 1030, 12001), 3), ((8200, 258, 6000), 0), ((4100, 256, 15000), 1),
+                                       ((768, 300, 60001), 0)])
+def test_gradient_by_parts(vh, sizes, pad):
+    """Sizes past the tiles' by a little, dx or dw in sums of several workgroups or whole, several pieces."""
+    Xent(vh, *sizes, 0.2, pad=pad, go=0.7).check()
+
+
 def test_several_pieces(vh):
-    """More rows than a piece holds: 512 rows a piece at this vocabulary."""
+    """More rows than a piece holds: 256 rows a piece at this vocabulary."""
     V = 400003
     assert vh.lib.vh_linear_cross_entropy_scratch_bytes(700, 8, V, 1) < 4 * 700 * V
     Xent(vh, 700, 8, V, 0.3).check()
@@ -99,7 +107,7 @@ def test_ignored(vh, ignore):
     Xent(vh, 10, 12, 9, ignore=ignore, t=t).check()
 
 
-@pytest.mark.parametrize("sizes", [(20, 8, 30), (400, 512, 2000)])
+@pytest.mark.parametrize("sizes", [(20, 8, 30), (400, 512, 2000), BIG])
 def test_no_row_counted(vh, sizes):
     c = Xent(vh, *sizes, t=[-100.0] * sizes[0])
     c.check()
@@ -108,16 +116,17 @@ def test_no_row_counted(vh, sizes):
 
 
 @pytest.mark.parametrize("scale", [1e-6, 30.0])
-@pytest.mark.parametrize("sizes", [(120, 64, 900), (400, 512, 2000)])
+@pytest.mark.parametrize("sizes", [(120, 64, 900), (400, 512, 2000), BIG])
 def test_flat_and_sharp(vh, scale, sizes):
     Xent(vh, *sizes, scale=scale).check()
 
 
-def test_rows_of_very_different_size(vh):
-    c = Xent(vh, 500, 600, 1500, 0.1, scale=0.05)
+@pytest.mark.parametrize("sizes", [(500, 600, 1500), BIG])
+def test_rows_of_very_different_size(vh, sizes):
+    c = Xent(vh, *sizes, 0.1, scale=0.05)
     r = np.random.default_rng(4)
-    c.x *= (10.0 ** r.uniform(-12, 0, (500, 1))).astype(np.float32)
-    c.w *= (10.0 ** r.uniform(-12, 0, (1500, 1))).astype(np.float32)
+    c.x *= (10.0 ** r.uniform(-12, 0, (sizes[0], 1))).astype(np.float32)
+    c.w *= (10.0 ** r.uniform(-12, 0, (sizes[2], 1))).astype(np.float32)
     c.x[7] = c.w[9] = 0
     c.put()
     c.check()
@@ -136,7 +145,7 @@ def test_bad_targets(vh, value, text):
     vh.sync()
 
 
-@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000), BIG])
 def test_bad_values_stay_in_their_row(vh, sizes):
     c = Xent(vh, *sizes)
     c.call("fwd")
@@ -153,7 +162,7 @@ def test_bad_values_stay_in_their_row(vh, sizes):
     np.testing.assert_array_equal(got["stats"][keep], clean["stats"][keep])
 
 
-@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000), BIG])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
 def test_ignored_rows_reach_nothing(vh, sizes, bad):
     """What a row that is not counted holds reaches neither the loss nor dw, and its dx is zero."""
@@ -171,7 +180,7 @@ def test_ignored_rows_reach_nothing(vh, sizes, bad):
         R.check(got, val, tol, ["loss", "dx", "dw"])
 
 
-@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000)])
+@pytest.mark.parametrize("sizes", [(40, 16, 200), (400, 512, 2000), BIG])
 @pytest.mark.parametrize("power", [-100, 100])
 def test_large_weights_of_small_rows(vh, sizes, power):
     """Logits of a usual size whose factors are far from one."""
@@ -183,13 +192,45 @@ def test_large_weights_of_small_rows(vh, sizes, power):
     R.check(c.results(), *R.linear_xent(c.x, c.w, c.t, c.ignore, c.go), ["loss", "stats"])
 
 
-def test_same_bits_and_streams(vh):
-    c = Xent(vh, 700, 64, 3001, 0.1)
+@pytest.mark.parametrize("go", [0.0, -3.0, 1e-20, 1e15])
+def test_gradients_of_the_loss(vh, go):
+    Xent(vh, *BIG, 0.1, go=go).check()
+
+
+def test_entries_of_small_probability(vh):
+    """Entries that no row gives weight: each row of dw to its own size, not to the largest one's."""
+    c = Xent(vh, *BIG)
+    V, rare = BIG[2], np.arange(5000, 5100)
+    c.w[:] *= 0.1
+    c.x[:, 0], c.w[:, 0] = 1, 0
+    c.w[rare, 0] = -np.linspace(20, 60, 100)
+    c.t = (c.t + 200 * ((c.t >= 5000) & (c.t < 5100))).astype(np.float32)
+    c.put()
+    val, tol = R.linear_xent(c.x, c.w, c.t, c.ignore, c.go)
+    # No entry here is a target, so dz is p / R with no difference taken: p to 4 e + (V + 16) u
+    # of itself, e the logit's error, and the sum over rows as everywhere.
+    x, w = R.f64(c.x), R.f64(c.w[rare])
+    p = torch.exp(x @ w.T - R.f64(val["stats"][:, :1])) / R.f64(val["stats"][:, 1:]) / BIG[0]
+    e = ((x.abs() @ w.abs().T) * (R.W + (BIG[1] + 4) * R.U)).amax()
+    small = (p.T @ x.abs()).numpy() * float(4 * e + (V + 16) * R.U + R.W + (BIG[0] + 4) * R.U)
+    assert (small < 0.1 * tol["dw"][rare]).all()
+    for calls in (("fwd", "bwd"), ("fwd_bwd",)):
+        c.put()
+        for which in calls:
+            c.call(which)
+        got = c.results()
+        R.check(got, val, tol, ["loss", "dx", "dw"])
+        assert (np.abs(got["dw"][rare] - val["dw"][rare]) <= small).all()
+
+
+@pytest.mark.parametrize("sizes", [(700, 64, 3001), BIG])
+def test_same_bits_and_streams(vh, sizes):
+    c = Xent(vh, *sizes, 0.1)
     c.call("fwd_bwd")
     want = c.results()
     st = Streams(2)
     try:
-        d = [Xent(vh, 700, 64, 3001, 0.1) for _ in range(2)]
+        d = [Xent(vh, *sizes, 0.1) for _ in range(2)]
         vh.sync()
         for rep in range(2):
             for x, s in zip(d, st.s):
@@ -203,7 +244,7 @@ def test_same_bits_and_streams(vh):
         st.close()
     with pytest.raises(vh.VhError, match="too small"):
         c.call("fwd", vh.DeviceBuffer(64))
-    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(700, 64, 3001, 1))
+    scratch = vh.DeviceBuffer(vh.lib.vh_linear_cross_entropy_scratch_bytes(*sizes, 1))
     c.call("fwd_bwd", scratch)
     np.testing.assert_array_equal(c.results()["dw"], want["dw"])
 

@@ -219,8 +219,8 @@ def test_scratch_sizes():
     assert L.vh_packed_attention_scratch_bytes(0, 1, 4, 2, 64, 1) == 0
     assert L.vh_packed_attention_scratch_bytes(16384, 8, 12, 4, 64, 1) >= 4 * 12 * 16384
     assert L.vh_qk_norm_rope_bwd_scratch_bytes(0, 64) == 0 < L.vh_qk_norm_rope_bwd_scratch_bytes(1, 1)
-    # A gradient's pieces: below the logits, and no less than 256 rows of them. A forward: none.
-    assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 1) < 4 * 65536 * 50257 // 8
+    # A gradient's pieces: three blocks of 683 MiB, and no less than 256 rows of logits. A forward: none.
+    assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 1) < 4 * 65536 * 50257 // 4
     assert L.vh_linear_cross_entropy_scratch_bytes(1024, 8, 4000000, 1) >= 4 * 256 * 4000000
     assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 0) < 4 * 65536 * 50257 // 16
     assert L.vh_linear_cross_entropy_scratch_bytes(0, 8, 8, 1) == 0
@@ -240,6 +240,7 @@ def test_code_object_holds_every_kernel():
     for dp in (32, 48, 64, 80, 96, 112, 128, 192, 256):
         names |= {f"vh_pa_{k}_{dp}" for k in ("prep", "fwd", "dq", "dkdv", "join")}
     names |= {f"vh_pa_bwd_{dp}" for dp in (32, 48, 64, 80, 96, 112, 128)}
-    names |= {"vh_lx_" + k for k in ("count", "stats", "grad", "stats_grad", "loss", "split", "logits", "finish")}
+    names |= {"vh_lx_" + k for k in ("count", "stats", "grad", "stats_grad", "loss", "split", "logits", "finish", "tops", "cols", "dz",
+                                   "mm", "join")}
     assert not names - elf_symbols(path)
     assert open(path, "rb").read() in open(vh.LIB_PATH, "rb").read()

@@ -38,3 +38,8 @@ extern "C" __global__ void __launch_bounds__(1024) vh_lx_loss(LxLossArgs a) { lx
 extern "C" __global__ void __launch_bounds__(256) vh_lx_split(LxSplitArgs a) { lx_split_impl(a); }
 extern "C" __global__ void __launch_bounds__(256, 2) vh_lx_logits(LxLogitArgs a) { lx_logits_impl(a); }
 extern "C" __global__ void __launch_bounds__(256) vh_lx_finish(LxFinishArgs a) { lx_finish_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_lx_tops(LxColsArgs a) { lx_tops_impl(a); }
+extern "C" __global__ void __launch_bounds__(512) vh_lx_cols(LxColsArgs a) { lx_cols_impl(a); }
+extern "C" __global__ void __launch_bounds__(512) vh_lx_dz(LxDzArgs a) { lx_dz_impl(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) vh_lx_mm(LxMmArgs a) { lx_mm_impl(a); }
+extern "C" __global__ void __launch_bounds__(256) vh_lx_join(LxMmArgs a) { lx_join_impl(a); }

@@ -232,23 +232,61 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
 }
 
 // ------------------------------------------------- cross-entropy of a linear layer --
-constexpr size_t kLxPieceBytes = size_t(1) << 30;
+constexpr size_t kLxPieceBytes = size_t(683) << 20;
 int64_t lx_ld(int64_t V) { return (V + 3) / 4 * 4; }
 // Logits by the f16 parts (vh_lx_logits) from this many multiply-adds on; below, the
 // splitting of both operands costs more than the products.
 constexpr double kLxLogits = 268435456.0;
 bool lx_by_parts(int64_t R, int64_t D, int64_t V) { return (double)R * (double)D * (double)V >= kLxLogits; }
+// The gradient's products by f16 parts too (vh_lx_mm): where the rows and the width fill its
+// tiles, and the fragments of w and dz are worth writing. Loss and gradient by it and by
+// vh_gemm: [2048, 768] x 50257 2.00 and 2.45 ms, [8192, 512] x 4000 519 and 567 us, [1500, 300]
+// x 30000 652 and 704; [4096, 256] x 10000 465 and 432, [8192, 128] x 16000 925 and 848, [512,
+// 768] x 50257 858 and 853.
+constexpr double kLxGrad = 1.2e10;
+bool lx_grad_by_parts(int64_t R, int64_t D, int64_t V) {
+  return (double)R * (double)D * (double)V >= kLxGrad && R >= 768 && D >= 256;
+}
 // Rows per piece: pieces of even size in whole 256-row product tiles, within kLxPieceBytes
-// of logits (one tile at least). The gradient's products want many rows: at [16384, 50257],
-// D = 768, pieces of 256 MB take 23.9 ms, 512 MB 22.0, 1 GB 20.7, 2 GB 20.0. A forward that
-// keeps no logits at all is one piece.
+// of logits (one tile at least; vh_lx_mm's operands take twice as much beside them). The
+// gradient's products want many rows: at [16384, 50257], D = 768, pieces of 341 MB take 16.3
+// ms, 512 MB 14.8, 683 MB 14.1, 1 GB 13.8. A forward that keeps no logits at all is one piece.
 int64_t lx_rows(int64_t R, int64_t D, int64_t V, bool backward) {
   if (!backward && lx_by_parts(R, D, V)) return R;
-  const int64_t fit = std::max<int64_t>((int64_t)(kLxPieceBytes / (sizeof(float) * (size_t)lx_ld(V))) / 256 * 256, 256);
+  int64_t fit = std::max<int64_t>((int64_t)(kLxPieceBytes / (sizeof(float) * (size_t)lx_ld(V))) / 256 * 256, 256);
+  if (lx_grad_by_parts(R, D, V)) fit = std::min<int64_t>(fit, 8192);  // (LX_DEEP's)
   return std::min<int64_t>(R, cdiv(cdiv(R, cdiv(R, fit)), 256) * 256);
 }
+// A product of fragments, M x N over ke steps of 16 k: how many of its tiles one workgroup
+// makes whole, and over how many the steps of each other tile go: what takes least, in
+// steps, of rounds of 512 workgroups (two a CU) and of the sums written and read (5 TB/s; a
+// step takes 0.7 us). 50257 x 768 is 1182 tiles: 2.3 rounds, of which the last is made 3.
+struct LxTiles {
+  int32_t tiles, tn, ke, full = 0, per, splits = 1;
+  LxTiles(int64_t M, int64_t N, int64_t steps)
+      : tiles((int32_t)std::min<int64_t>(cdiv(M, VH_LX_TV) * cdiv(N, VH_LX_TR), INT32_MAX)),
+        tn((int32_t)cdiv(N, VH_LX_TR)), ke((int32_t)steps), per(ke) {
+    double best = 1e300;
+    for (int32_t f = tiles / 512; f >= 0 && f >= tiles / 512 - 1; --f)
+      for (int32_t s = 1; s <= 16; ++s) {
+        const int32_t p = (int32_t)cdiv(cdiv(ke, s), 16) * 16, n = (int32_t)cdiv(ke, p), rest = tiles - 512 * f;
+        const double sums = n > 1 ? (double)rest * (n + 1) * (4.0 * VH_LX_TV * VH_LX_TR / 3.5e6) : 0.0;
+        const double t = (double)f * ke + (double)cdiv((int64_t)rest * n, 512) * std::min(p, ke) + sums;
+        if (t < best) {
+          best = t;
+          full = 512 * f;
+          per = p;
+          splits = n;
+        }
+      }
+  }
+  size_t sums() const {
+    return splits > 1 ? sizeof(float) * (size_t)splits * (size_t)(tiles - full) * VH_LX_TV * VH_LX_TR : 0;
+  }
+};
+
 struct LxScratch {
-  size_t z, xs, row_loss, inv, stats, xf, xe, wf, we, part, zt, total;
+  size_t z, top, re, zr, zc, ce, xt, wt, xs, row_loss, inv, stats, xf, xe, wf, we, part, zt, total;
   LxScratch(int64_t R, int64_t D, int64_t V, bool backward) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -258,8 +296,19 @@ struct LxScratch {
     };
     const bool parts = lx_by_parts(R, D, V);
     const int64_t rows = lx_rows(R, D, V, backward);
-    z = take(parts && !backward ? 0 : sizeof(float) * (size_t)(rows * lx_ld(V)));
-    xs = take(backward ? sizeof(float) * (size_t)(rows * lx_ld(D)) : 0);
+    const bool grad = backward && lx_grad_by_parts(R, D, V);
+    const size_t vb = (size_t)cdiv(V, 32), rb = (size_t)cdiv(rows, 256), db = (size_t)cdiv(D, 32);
+    // (The products' sums lie where z did.)
+    const size_t sums = grad ? std::max(LxTiles(rows, D, (int64_t)vb * 2).sums(), LxTiles(V, D, (int64_t)rb * 16).sums()) : 0;
+    z = take(std::max(parts && !backward ? 0 : sizeof(float) * (size_t)(rows * lx_ld(V)), sums));
+    top = take(grad ? 2 * sizeof(uint32_t) * (size_t)D : 0);  // column maxima of w, of x
+    re = take(grad ? sizeof(int32_t) * 256 * rb : 0);
+    zr = take(grad ? rb * 8 * vb * 2 * 2048 : 0);  // dz by rows, by columns, and the columns' exponents
+    zc = take(grad ? vb * rb * 16 * 2048 : 0);
+    ce = take(grad ? sizeof(int32_t) * rb * vb * 32 : 0);
+    xt = take(grad ? db * rb * 16 * 2048 : 0);
+    wt = take(grad ? db * vb * 2 * 2048 : 0);
+    xs = take(backward && !grad ? sizeof(float) * (size_t)(rows * lx_ld(D)) : 0);
     row_loss = take(sizeof(float) * (size_t)R);
     inv = take(256);
     stats = take(backward ? 2 * sizeof(float) * (size_t)R : 0);  // (of a call that returns none)
@@ -338,7 +387,34 @@ int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes,
                         aligned16(p) && stride % 4 == 0 && c.D % 4 == 0};
     return launch("vh_lx_split", cdiv(rows, 32), 1, 1, 256, s, a);
   };
-  VH_TRY(launch("vh_lx_count", 1, 1, 1, 1024, s, LxCountArgs{c.targets, inv, vh_rt::error_record(), c.R, V, c.ignore}));
+  const bool grad = c.backward && lx_grad_by_parts(c.R, c.D, c.V);
+  const int32_t D = (int32_t)c.D, kv = (int32_t)(cdiv(c.V, 32) * 2);
+  uint32_t* top = reinterpret_cast<uint32_t*>(base + lay.top);
+  VH_TRY(launch("vh_lx_count", 1, 1, 1, 1024, s,
+                LxCountArgs{c.targets, inv, top, grad ? 2 * c.D : 0, vh_rt::error_record(), c.R, V, c.ignore}));
+  // A matrix's columns as fragments of column powers of two.
+  auto tops = [&](const float* p, const float* t, int64_t stride, int64_t rows, uint32_t* to) {
+    return launch("vh_lx_tops", cdiv(rows, 256), cdiv(c.D, 64), 1, 256, s, LxColsArgs{p, t, to, nullptr, rows, stride, D, 0, c.ignore});
+  };
+  auto cols = [&](const float* p, const float* t, int64_t stride, int64_t rows, uint32_t* from, size_t f, int64_t k) {
+    return launch("vh_lx_cols", cdiv(rows, 256), cdiv(c.D, 32), 1, 512, s,
+                  LxColsArgs{p, t, from, frags(f), rows, stride, D, (int32_t)k, c.ignore});
+  };
+  // out [M, D] (+)= a b^T
+  auto product = [&](int64_t M, size_t af, size_t ae, int64_t ae_step, size_t bf, uint32_t* btop, int64_t steps, float* out,
+                     int64_t ldo, bool add) {
+    const LxTiles t(M, c.D, steps);
+    const LxMmArgs m{frags(af), frags(bf), exps(ae), btop,  out,  z,      M,        ldo,
+                     ae_step,   D,         t.ke,     t.per, t.tiles, t.tn, t.full, t.splits, add};
+    const int64_t rest = t.tiles - t.full;
+    VH_TRY(launch("vh_lx_mm", t.full + cdiv(rest * t.splits, 8) * 8, 1, 1, 256, s, m));
+    return t.splits > 1 ? launch("vh_lx_join", rest, VH_LX_TV / 8, 1, 256, s, m) : VH_OK;
+  };
+  if (grad) {
+    VH_TRY(tops(c.w, nullptr, c.ldw, c.V, top));
+    VH_TRY(tops(c.x, c.targets, c.ldx, c.R, top + c.D));
+    VH_TRY(cols(c.w, nullptr, c.ldw, c.V, top, lay.wt, kv));
+  }
   if (parts) VH_TRY(split(c.w, c.ldw, c.V, lay.wf, lay.we));
   for (int64_t r = 0; r < c.R; r += piece) {
     const int64_t rows = std::min(piece, c.R - r);
@@ -350,11 +426,22 @@ int lx_run(const char* fn, const LxCall& c, void* scratch, size_t scratch_bytes,
       const LxLogitArgs a{frags(lay.wf), exps(lay.we), frags(lay.xf), exps(lay.xe), t, c.forward ? at(lay.part) : nullptr,
                           at(lay.zt), c.backward ? z : nullptr, rows, ld, V, ke, tv, tr, c.ignore};
       VH_TRY(launch("vh_lx_logits", cdiv((int64_t)tv * tr, 8) * 8, 1, 1, 256, s, a));
-      if (c.forward)
+      if (c.forward || grad)
         VH_TRY(launch("vh_lx_finish", cdiv(rows, 4), 1, 1, 256, s,
-                      LxFinishArgs{at(lay.part), at(lay.zt), t, st, row_loss + r, rows, V, tv, c.ignore}));
+                      LxFinishArgs{c.forward ? at(lay.part) : nullptr, at(lay.zt), t, c.grad_out, inv, st, row_loss + r,
+                                   grad ? exps(lay.re) : nullptr, rows, V, tv, c.ignore}));
     } else {
       VH_TRY(lx_product(rows, c.V, c.D, x, c.ldx, 1, c.w, 1, c.ldw, z, ld, false, s));
+    }
+    if (grad) {
+      const int64_t rb = cdiv(rows, 256), vs = cdiv(c.V, 32);
+      VH_TRY(cols(x, t, c.ldx, rows, top + c.D, lay.xt, rb * 16));
+      VH_TRY(launch("vh_lx_dz", vs, rb, 1, 512, s,
+                    LxDzArgs{z, t, c.grad_out, inv, st, exps(lay.re), frags(lay.zr), frags(lay.zc), exps(lay.ce), rows, ld,
+                             vs * 32, V, kv, (int32_t)rb * 16, c.ignore}));
+      VH_TRY(product(rows, lay.zr, lay.re, 0, lay.wt, top, kv, c.dx + r * c.lddx, c.lddx, false));
+      VH_TRY(product(c.V, lay.zc, lay.ce, vs * 32, lay.xt, top + c.D, rb * 16, c.dw, c.lddw, r > 0));
+      continue;
     }
     const char* kernel = parts || !c.forward ? "vh_lx_grad" : c.backward ? "vh_lx_stats_grad" : "vh_lx_stats";
     if (c.backward || !parts)

@@ -522,6 +522,8 @@ struct LxArgs {
 struct LxCountArgs {
   const float* targets;
   float* inv;
+  uint32_t* zero;        // nzero words to clear
+  int64_t nzero;
   VhErrRecord* err;
   int64_t R;
   int32_t V;
@@ -549,7 +551,7 @@ struct LxLogitArgs {
   const int32_t* xe;
   const float* targets;  // of the rows
   float* part;           // [rows][tiles of entries][2] max, sum of exp; null: not wanted
-  float* zt;             // [rows] the target's logit (with part)
+  float* zt;             // [rows] the target's logit
   float* z;              // [rows, ld] logits, or null
   int64_t rows, ld;
   int32_t V, ke;
@@ -560,9 +562,51 @@ struct LxFinishArgs {
   const float* part;
   const float* zt;
   const float* targets;
+  const float* grad_out; // with exp
+  const float* inv;
   float* stats;
   float* row_loss;
+  int32_t* exp;          // [rows] exponents of the rows' gradients, or null
   int64_t rows;
   int32_t V, tv;
   float ignore;
+};
+// The gradient's products by f16 parts. Column maxima of K rows of D (bits of |x|, rows that
+// are not counted left out where there are targets), and those columns as fragments.
+struct LxColsArgs {
+  const float* x;
+  const float* targets;  // of the rows, or null: all count
+  uint32_t* top;         // [D]
+  uint16_t* frag;        // [32 columns][16 rows][part][64 pieces of 8]
+  int64_t rows, ld;
+  int32_t D, ke;
+  float ignore;
+};
+// A piece's logits to their gradient as fragments: by rows (for dx) and by columns (for dw).
+struct LxDzArgs {
+  const float* z;
+  const float* targets;
+  const float* grad_out;
+  const float* inv;
+  const float* stats;
+  const int32_t* exp;    // [rows]
+  uint16_t* by_row;      // [32 rows][16 entries]..., kv of 16
+  uint16_t* by_col;      // [32 entries][16 rows]..., kr of 16
+  int32_t* col_exp;      // [256 rows][cols]
+  int64_t rows, ld, cols;
+  int32_t V, kv, kr;
+  float ignore;
+};
+// out[m, n] = sum over k of a[m, k] b[n, k], fragments both. The first `full` tiles are made
+// whole, each of the others in `splits` sums of `per` steps of 16 k that LxJoinArgs adds.
+struct LxMmArgs {
+  const uint16_t* a;
+  const uint16_t* b;
+  const int32_t* ae;     // [m] exponents; every 16 steps another ae_step on
+  const uint32_t* btop;  // [n] largest values (bits), whose exponents b's are
+  float* out;            // [m, n]
+  float* part;           // [split][tile past full][256][128]
+  int64_t M, ld, ae_step;  // ae_step 0: the same exponents for all k
+  int32_t N, ke, per;
+  int32_t tiles, tn, full, splits, add;  // tn: tiles along n, the faster
 };
