@@ -88,6 +88,43 @@ def test_parts_of_the_query_heads(vh, Hq, Hk, L):
     run_and_check(vh, [L] * (16384 // L), Hq, Hk, 32, True, seed=L)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,Hq,Hk,D", [([1100], 1, 1, 32), ([257, 1, 900], 2, 1, 48), ([1000, 129], 3, 1, 64), ([513], 3, 3, 80),
+                                          ([640, 384], 4, 2, 112), ([700], 2, 1, 128), ([600], 2, 2, 192), ([385], 1, 1, 250)])
+def test_few_rows(vh, lens, Hq, Hk, D, causal):
+    """Blocks whose keys, and whose queries, are divided over workgroups, with blocks too short for it beside them."""
+    run_and_check(vh, lens, Hq, Hk, D, causal, seed=D, first=5, tail=7, kinds=("plain",) * 4)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_with_bad_values(vh, bad, D):
+    """A key that only later rows see, of a block divided over workgroups: rows before it as without it."""
+    lens, at = [900], 610
+    a = inputs(lens, 2, 1, D, 23)
+    b = [x.copy() for x in a]
+    b[1][at], b[2][at] = bad, bad
+    got = R.Attention(vh, *b, R.starts_of(lens), 0.1, True).run()
+    val, tol = R.attention(*(x[:at] for x in a), [at], 0.1, True)
+    for n in ("o", "dq"):
+        assert (np.abs(got[n][:at] - val[n]) <= tol[n]).all(), n
+    assert (np.abs(got["lse"][:, :at] - val["lse"]) <= tol["lse"]).all()
+    if np.isnan(bad):
+        assert np.isnan(got["o"][at:]).all() and np.isnan(got["dq"][at:]).all()
+
+
+def test_few_rows_one_chunk_of_no_weight(vh):
+    """Scores of -infinity through one whole chunk: its keys have no weight, and nothing of them is seen."""
+    lens, D = [600], 64
+    q, k, v, do = inputs(lens, 1, 1, D, 25)
+    q[..., 0] = 1.0
+    k[:200, 0, 0] = -np.inf
+    val, tol = R.attention(q[200:], k[200:], v[200:], do[200:], [400], 0.1, False)
+    got = R.Attention(vh, q, k, v, do, R.starts_of(lens), 0.1, False).run()
+    assert (np.abs(got["o"][200:] - val["o"]) <= tol["o"]).all()
+    assert (np.abs(got["lse"][:, 200:] - val["lse"]) <= tol["lse"]).all()
+
+
 def test_broadcast_keys(vh):
     """Every token and head reading one key row (zero strides): its gradient comes out per row."""
     lens, Hq, Hk, D = [40, 90], 4, 2, 64
@@ -225,16 +262,22 @@ def test_sharp_scores(vh):
 
 @pytest.mark.parametrize("D", [64, 128, 160])
 def test_same_bits_and_no_neighbours(vh, D):
-    """Twice the same bits, and a sequence's results do not depend on its neighbours or its place."""
+    """Twice the same bits, whatever the tokens of other sequences are. (How sums are grouped goes by the batch's sizes.)"""
     lens = [130, 77, 200]
     a = inputs(lens, 4, 2, D, 17)
     one = R.Attention(vh, *a, R.starts_of(lens), 0.1, True).run()
     two = R.Attention(vh, *a, R.starts_of(lens), 0.1, True).run()
     s = slice(130, 207)
-    alone = R.Attention(vh, *(x[s] for x in a), [0, 77], 0.1, True).run()
+    others = [x.copy() for x in a]
+    for x in others:
+        x[:130], x[207:] = x[:130][::-1] * 3, x[207:][::-1] * 0.5
+    among = R.Attention(vh, *others, R.starts_of(lens), 0.1, True).run()
+    val, tol = R.attention(*(x[s] for x in a), [77], 0.1, True)
+    R.check(R.Attention(vh, *(x[s] for x in a), [0, 77], 0.1, True).run(), val, tol)
     for n in one:
         np.testing.assert_array_equal(one[n], two[n], err_msg=n)
-        np.testing.assert_array_equal(one[n][:, s] if n == "lse" else one[n][s], alone[n], err_msg=n)
+        cut = (lambda y: y[:, s]) if n == "lse" else (lambda y: y[s])
+        np.testing.assert_array_equal(cut(one[n]), cut(among[n]), err_msg=n)
 
 
 def test_gradients_against_differences(vh):

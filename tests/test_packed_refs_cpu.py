@@ -238,7 +238,7 @@ def test_code_object_holds_every_kernel():
     names = {f"vh_rope_{d}_v{c}" for d in ("fwd", "bwd") for c in ("4_l4_n1", "4_l8_n1", "4_l16_n1", "4_l32_n1", "1_l64_n1",
                                                                   "1_l64_n2")}
     for dp in (32, 48, 64, 80, 96, 112, 128, 192, 256):
-        names |= {f"vh_pa_{k}_{dp}" for k in ("prep", "fwd", "dq", "dkdv", "join")}
+        names |= {f"vh_pa_{k}_{dp}" for k in ("prep", "fwd", "fold", "dq", "dkdv", "join")}
     names |= {f"vh_pa_bwd_{dp}" for dp in (32, 48, 64, 80, 96, 112, 128)}
     names |= {"vh_lx_" + k for k in ("count", "stats", "grad", "stats_grad", "loss", "split", "logits", "finish", "tops", "cols", "dz",
                                    "mm", "join")}

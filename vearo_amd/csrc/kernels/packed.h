@@ -126,6 +126,17 @@ VH_DEV void pa_tables(const PaArgs& a, int idx, PaFind& f) {
   }
 }
 
+// Where rows are few, a block's steps of 32 keys are divided over a.chunks workgroups: how many
+// steps each takes (four at least), and how many of them some row of the 32 from r0 on sees.
+VH_DEV int pa_steps(const PaArgs& a, const PaSpan& sp, int r0, int rows) {
+  return ((a.causal ? min(sp.len, r0 + rows) : sp.len) + 31) >> 5;
+}
+VH_DEV int pa_chunk(const PaArgs& a, const PaSpan& sp, int row0) {
+  const int nt = pa_steps(a, sp, row0, a.block_rows);
+  return a.chunks > 1 ? max(4, (nt + a.chunks - 1) / a.chunks) : nt;
+}
+VH_DEV int64_t pa_fold_at(const PaArgs& a, int chunk, int64_t tok, int h) { return (((int64_t)chunk * a.T + tok) * a.q.H + h) * a.DP; }
+
 // -------------------------------------------------------------- row forms --
 // A wave per row, keys over its lanes for the scores, elements over its lanes for
 // the products. Scores are formed again in each pass instead of kept, so a row may
@@ -160,41 +171,56 @@ VH_DEV void pa_axpy(float c, const float* x, int64_t st, int m, int D, float (&a
   }
 }
 
-VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l) {
+// (Forward and dq: over keys 32 c0 .. 32 c1 - 1.)
+VH_DEV void pa_row_fwd(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l, int c0, int c1, int chunk) {
   const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
   const int64_t tok = (int64_t)sp.start + i;
   const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
   const float* v = a.v.p + sp.start * a.v.st + hk * a.v.sh;
-  const int nk = a.causal ? i + 1 : sp.len;
+  const int nk = min(a.causal ? i + 1 : sp.len, 32 * c1);
+  if (32 * c0 >= nk) return;
   pa_row_to_lds(l, a.q.p + tok * a.q.st + h * a.q.sh, a.D);
   float m = -INFINITY;
-  for (int j = lane; j < nk; j += 64) m = fmaxf(m, pa_dot(l, k + j * a.k.st, a.D) * a.scale);
+  for (int j = 32 * c0 + lane; j < nk; j += 64) m = fmaxf(m, pa_dot(l, k + j * a.k.st, a.D) * a.scale);
   m = group_max<64>(m);
+  // (A chunk of scores of -infinity alone has no weight beside another's.)
+  const float mb = a.chunks > 1 && m == -INFINITY ? 0.0f : m;
   float sum = 0.0f, acc[4] = {};
-  for (int j0 = 0; j0 < nk; j0 += 64) {
+  for (int j0 = 32 * c0; j0 < nk; j0 += 64) {
     float p = 0.0f;
-    if (j0 + lane < nk) p = expf(pa_dot(l, k + (j0 + lane) * a.k.st, a.D) * a.scale - m);
+    if (j0 + lane < nk) p = expf(pa_dot(l, k + (j0 + lane) * a.k.st, a.D) * a.scale - mb);
     sum += p;
     pa_axpy(p, v + j0 * a.v.st, a.v.st, min(64, nk - j0), a.D, acc);
   }
   sum = group_sum<64>(sum);
+  if (a.chunks > 1) {
+    float* o = a.fold + pa_fold_at(a, chunk, tok, h);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (lane + 64 * u < a.D) o[lane + 64 * u] = sum == 0.0f ? 0.0f : acc[u] / sum;
+    if (lane == 0)  // (in the matrix kernels' units)
+      *reinterpret_cast<float2*>(a.fold_ml + 2 * (((int64_t)chunk * a.q.H + h) * a.T + tok)) =
+          make_float2(m * 1.4426950408889634f, sum * 16384.0f);
+    return;
+  }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (lane + 64 * u < a.D) a.out[tok * a.out_t + h * a.out_h + lane + 64 * u] = acc[u] / sum;
   if (lane == 0) a.lse[(int64_t)h * a.T + tok] = m + logf(sum);
 }
 
-VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l, PaLds lg) {
+VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l, PaLds lg, int c0, int c1, int chunk) {
   const int lane = threadIdx.x & 63, hk = h / (a.q.H / a.k.H);
   const int64_t tok = (int64_t)sp.start + i;
   const float* k = a.k.p + sp.start * a.k.st + hk * a.k.sh;
   const float* v = a.v.p + sp.start * a.v.st + hk * a.v.sh;
-  const int nk = a.causal ? i + 1 : sp.len;
+  const int nk = min(a.causal ? i + 1 : sp.len, 32 * c1);
+  if (32 * c0 >= nk) return;
   pa_row_to_lds(l, a.q.p + tok * a.q.st + h * a.q.sh, a.D);
   pa_row_to_lds(lg, a.g.p + tok * a.g.st + h * a.g.sh, a.D);
   const float lse = a.lse[(int64_t)h * a.T + tok], dl = a.delta[(int64_t)h * a.T + tok];
   float acc[4] = {};
-  for (int j0 = 0; j0 < nk; j0 += 64) {
+  for (int j0 = 32 * c0; j0 < nk; j0 += 64) {
     float ds = 0.0f;
     if (const int64_t j = j0 + lane; j < nk) {
       const float p = expf(pa_dot(l, k + j * a.k.st, a.D) * a.scale - lse);
@@ -202,9 +228,10 @@ VH_DEV void pa_row_dq(const PaArgs& a, int h, const PaSpan& sp, int i, PaLds l, 
     }
     pa_axpy(ds, k + j0 * a.k.st, a.k.st, min(64, nk - j0), a.D, acc);
   }
+  float* o = a.chunks > 1 ? a.fold + pa_fold_at(a, chunk, tok, h) : a.dq + tok * a.dq_t + h * a.dq_h;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (lane + 64 * u < a.D) a.dq[tok * a.dq_t + h * a.dq_h + lane + 64 * u] = acc[u] * a.scale;
+    if (lane + 64 * u < a.D) o[lane + 64 * u] = acc[u] * a.scale;
 }
 
 // Over query heads h0 .. h1 - 1, into dk and dv or, of several parts, into this one's sums.
@@ -243,16 +270,16 @@ VH_DEV void pa_row_dkdv(const PaArgs& a, int hk, const PaSpan& sp, int j, PaLds 
     }
 }
 
-// The rows of one block, over the workgroup's waves. MODE 0 forward, 1 dq, 2 dk and dv.
+// The rows of one block, over the workgroup's waves. MODE 0 forward, 1 dq (over steps c0 ..
+// c1 - 1 of 32 keys), 2 dk and dv (over query heads c0 .. c1 - 1).
 template <int MODE>
-VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, PaLds l, int h0 = 0, int h1 = 0,
-                    int part = 0) {
+VH_DEV void pa_rows(const PaArgs& a, int h, const PaSpan& sp, PaLds l, int c0, int c1, int part) {
   const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int end = min(sp.len, sp.row0 + a.block_rows);
   l += w * 2 * VH_PA_MAX_D;  // the wave's two rows
   for (int i = sp.row0 + w; i < end; i += nw) {
-    if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l);
-    if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l, l + VH_PA_MAX_D);
-    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l, l + VH_PA_MAX_D, h0, h1, part);
+    if constexpr (MODE == 0) pa_row_fwd(a, h, sp, i, l, c0, c1, part);
+    if constexpr (MODE == 1) pa_row_dq(a, h, sp, i, l, l + VH_PA_MAX_D, c0, c1, part);
+    if constexpr (MODE == 2) pa_row_dkdv(a, h, sp, i, l, l + VH_PA_MAX_D, c0, c1, part);
   }
 }

@@ -22,7 +22,8 @@ K_ROPE(4, 4, 1) K_ROPE(4, 8, 1) K_ROPE(4, 16, 1) K_ROPE(4, 32, 1) K_ROPE(1, 64, 
   extern "C" __global__ void __launch_bounds__(256, W1) vh_pa_fwd_##DP(PaArgs a) { pa_mm_fwd_impl<DP, 4>(a); }    \
   extern "C" __global__ void __launch_bounds__(256, W2) vh_pa_dq_##DP(PaArgs a) { K_PA_LDS(DP) pa_mm_dq_impl<DP, 4>(a, blockIdx.x, lds); } \
   extern "C" __global__ void __launch_bounds__(256, W3) vh_pa_dkdv_##DP(PaArgs a) { K_PA_LDS(DP) pa_mm_dkdv_impl<DP, 4, HALVES>(a, blockIdx.x, lds); } \
-  extern "C" __global__ void __launch_bounds__(256) vh_pa_join_##DP(PaArgs a) { pa_join_impl<DP>(a); }
+  extern "C" __global__ void __launch_bounds__(256) vh_pa_join_##DP(PaArgs a) { pa_join_impl<DP>(a); } \
+  extern "C" __global__ void __launch_bounds__(256) vh_pa_fold_##DP(PaArgs a) { pa_fold_impl<DP>(a); }
 K_PA(32, 4, 4, 3, 1) K_PA(48, 3, 3, 2, 1) K_PA(64, 3, 3, 2, 1) K_PA(80, 2, 2, 1, 1) K_PA(96, 2, 2, 1, 1)
 K_PA(112, 2, 1, 1, 1) K_PA(128, 2, 1, 1, 1) K_PA(192, 1, 1, 1, 2) K_PA(256, 1, 1, 1, 2)
 #define K_PA_BWD(DP, W) \

@@ -416,11 +416,12 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * SUB];  // two stages of K, of V
   const PaHalves lk = (PaHalves)lds, lv = lk + 2 * SUB;
   const int H = a.q.H, id = blockIdx.x;
-  const PaSpan sp = a.blocks[id / H];  // (inside the table, also where it is not written)
-  if (id >= a.head->nblocks * H) return;
-  const int h = id % H, hk = h / (H / a.k.H);
+  const PaSpan sp = a.blocks[id / (H * a.chunks)];  // (inside the table, also where it is not written)
+  if (id / (H * a.chunks) >= a.head->nblocks) return;
+  const int part = id % a.chunks, h = id / a.chunks % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
-  const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
+  const int all = pa_steps(a, sp, sp.row0, 32 * NW), per = pa_chunk(a, sp, sp.row0), c0 = part * per, nt = min(c0 + per, all);
+  if (c0 >= nt) return;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
   const PaStage<DP> fk(lk), fv(lv);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
@@ -428,18 +429,18 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   auto stage = [&](const uint16_t* p, int t, PaHalves to) {
     pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
   };
-  stage(sk.n, 0, lk);
-  stage(sv.n, 0, lv);
-  if (nt > 1) stage(sk.n, 1, lk + SUB);
+  stage(sk.n, c0, lk + (c0 & 1) * SUB);
+  stage(sv.n, c0, lv + (c0 & 1) * SUB);
+  if (nt > c0 + 1) stage(sk.n, c0 + 1, lk + (~c0 & 1) * SUB);
   PaFrag q[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q);
   PaRange rk, rv;
-  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk, rv);
+  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((all + 1) >> 1), rk, rv);  // (a block's chunks decide alike)
   rv.slow |= rk.slow;
   int top;
   if (rv.any_slow(top)) {
     pa_arrived();  // (nothing on its way into the rows' LDS)
-    pa_rows<0>(a, h, sp, (PaLds)lk);
+    pa_rows<0>(a, h, sp, (PaLds)lk, c0, nt, part);
     return;
   }
   const int lim = a.causal ? min(i, sp.len - 1) : sp.len - 1;
@@ -450,13 +451,13 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
   float m = -INFINITY, l = 0.0f;
   int ev = 0;
   // Steps that some row of the wave sees: all but the last are seen whole.
-  const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
+  const int mine = r0 >= sp.len ? 0 : min(pa_steps(a, sp, r0, 32), nt);
   // The steps' exponents, read one step ahead.
   const PaInfo ik = pa_info(sk.info) + ((int64_t)sp.tile0 * a.k.H + hk), iv = pa_info(sv.info) + ((int64_t)sp.tile0 * a.k.H + hk);
-  int ekn = *ik, evn = *iv;
+  int ekn = ik[(int64_t)(c0 >> 1) * a.k.H], evn = iv[(int64_t)(c0 >> 1) * a.k.H];
   // Step t's V and step t + 1's K are in LDS; V of t + 1 and K of t + 2 go out.
   auto arrive = [&](int t) {
-    if (t) pa_arrived();
+    if (t != c0) pa_arrived();
     if (t + 1 < nt) stage(sv.n, t + 1, lv + ((t + 1) & 1) * SUB);
     if (t + 2 < nt) stage(sk.n, t + 2, lk + (t & 1) * SUB);
   };
@@ -500,12 +501,12 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
     s = next;
   };
   pa_arrived();
-  if (mine > 0) {
+  if (mine > c0) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) pa_mma(fk.rows(0, k), q[k], s);
+    for (int k = 0; k < KS; ++k) pa_mma(fk.rows(c0 & 1, k), q[k], s);
   }
-  __syncthreads();  // (K of step 0 has been read)
-  int t = 0;
+  __syncthreads();  // (K of the first step has been read)
+  int t = c0;
   for (; t + 1 < mine; ++t) {
     arrive(t);
     step(t, std::false_type{});
@@ -515,14 +516,55 @@ VH_DEV void pa_mm_fwd_impl(const PaArgs& a) {
     step(t++, std::true_type{});
   }
   for (; t < nt; ++t) arrive(t);
-  if (r0 >= sp.len) return;
+  if (mine <= c0) return;
   l = pa_sum_halves(l);
   if (i >= sp.len) return;
   const int64_t tok = (int64_t)sp.start + i;
   const float inv = 1.0f / l;
+  if (a.chunks > 1) {
+    pa_store<DB>(a.fold + pa_fold_at(a, part, tok, h), 1, DP, o, [&](float v) { return pa_ldexp(v * inv, ev - PA_E); });
+    if (hf == 0) *reinterpret_cast<float2*>(a.fold_ml + 2 * (((int64_t)part * H + h) * a.T + tok)) = make_float2(m, l);
+    return;
+  }
   pa_store<DB>(a.out + tok * a.out_t + h * a.out_h, a.out_vec, a.D, o,
                [&](float v) { return pa_ldexp(v * inv, ev - PA_E); });
   if (hf == 0) a.lse[(int64_t)h * a.T + tok] = fmaf(m, PA_LN2, fmaf(m, PA_LN2_LO, logf(pa_ldexp(l, -PA_E))));
+}
+
+// A row's chunks brought together: out = sum of w o / sum of w, w = l 2^(m - max). Grid:
+// (tiles, query heads).
+template <int DP>
+VH_DEV void pa_fold_impl(const PaArgs& a) {
+  if ((int)blockIdx.x >= a.head->ntiles) return;
+  const PaSpan sp = a.tiles[blockIdx.x];
+  const int h = blockIdx.y, rows = min(64, sp.len - sp.row0);
+  const int per = pa_chunk(a, sp, sp.row0 / a.block_rows * a.block_rows);
+  for (int u = threadIdx.x; u < rows * (DP / 4); u += 256) {
+    const int row = sp.row0 + u / (DP / 4), d = u % (DP / 4) * 4;
+    const int used = (pa_steps(a, sp, row & ~31, 32) + per - 1) / per;
+    const int64_t tok = (int64_t)sp.start + row;
+    const float2* ml = reinterpret_cast<const float2*>(a.fold_ml) + (int64_t)h * a.T + tok;
+    const int64_t step = (int64_t)a.q.H * a.T;
+    float m = -INFINITY, l = 0.0f;
+    for (int c = 0; c < used; ++c) m = fmaxf(m, ml[c * step].x);
+    pa_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < used; ++c) {
+      const float2 x = ml[c * step];
+      const float w = x.y * __builtin_amdgcn_exp2f(x.x - m);
+      l += w;
+      s += *reinterpret_cast<const pa_f4*>(a.fold + pa_fold_at(a, c, tok, h) + d) * w;
+    }
+    s *= 1.0f / l;
+    float* o = a.out + tok * a.out_t + h * a.out_h + d;
+    if (a.out_vec) {
+      if (d < a.D) *reinterpret_cast<pa_f4*>(o) = s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < a.D) o[e] = s[e];
+    }
+    if (d == 0) a.lse[(int64_t)h * a.T + tok] = fmaf(m, PA_LN2, fmaf(m, PA_LN2_LO, logf(pa_ldexp(l, -PA_E))));
+  }
 }
 
 // -------------------------------------------------------------------- backward --
@@ -561,11 +603,12 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, PaHalves lds) {
   constexpr int KS = DP / 16, DB = (DP + 31) / 32, SUB = 64 * DP;
   const PaHalves lk = lds, lv = lds + 2 * SUB;
   const int H = a.q.H;
-  const PaSpan sp = a.blocks[id / H];
-  if (id >= a.head->nblocks * H) return;
-  const int h = id % H, hk = h / (H / a.k.H);
+  const PaSpan sp = a.blocks[id / (H * a.chunks)];
+  if (id / (H * a.chunks) >= a.head->nblocks) return;
+  const int part = id % a.chunks, h = id / a.chunks % H, hk = h / (H / a.k.H);
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
-  const int nt = ((a.causal ? min(sp.len, sp.row0 + 32 * NW) : sp.len) + 31) >> 5;
+  const int all = pa_steps(a, sp, sp.row0, 32 * NW), per = pa_chunk(a, sp, sp.row0), c0 = part * per, nt = min(c0 + per, all);
+  if (c0 >= nt) return;
   const PaStream &sk = a.stream[0], &sv = a.stream[1];
   const PaStage<DP> fk(lk), fv(lv);
   const int r0 = sp.row0 + 32 * w, i = r0 + (lane & 31);
@@ -574,17 +617,17 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, PaHalves lds) {
   auto stage = [&](const uint16_t* p, int t, PaHalves to) {
     pa_copy<NW, 2 * SUB>(p + base + (t >> 1) * chunk + (t & 1) * SUB, to);
   };
-  stage(sk.n, 0, lk);
-  stage(sv.n, 0, lv);
+  stage(sk.n, c0, lk + (c0 & 1) * SUB);
+  stage(sv.n, c0, lv + (c0 & 1) * SUB);
   PaFrag q[KS], gq[KS];
   const int eq = pa_own<DP>(a.q, sp, a.D, i, h, q), eg = pa_own<DP>(a.g, sp, a.D, i, h, gq);
   PaRange rk, rv;
-  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((nt + 1) >> 1), rk, rv);
+  pa_scan(sk, sv, a.k.H, hk, sp.tile0, sp.tile0 + ((all + 1) >> 1), rk, rv);
   rk.slow |= rv.slow;
   int top;
   if (rk.any_slow(top)) {
     pa_arrived();
-    pa_rows<1>(a, h, sp, (PaLds)lk);
+    pa_rows<1>(a, h, sp, (PaLds)lk, c0, nt, part);
     return;
   }
   const int64_t tok = (int64_t)sp.start + i;
@@ -596,10 +639,10 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, PaHalves lds) {
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = pa_f16{};
   int g = 126;
-  const int mine = r0 >= sp.len ? 0 : ((a.causal ? min(r0 + 32, sp.len) : sp.len) + 31) >> 5;
+  const int mine = r0 >= sp.len ? 0 : min(pa_steps(a, sp, r0, 32), nt);
   const PaInfo ik = pa_info(sk.info) + ((int64_t)sp.tile0 * a.k.H + hk), iv = pa_info(sv.info) + ((int64_t)sp.tile0 * a.k.H + hk);
-  int ekn = *ik, evn = *iv;
-  for (int t = 0; t < nt; ++t) {
+  int ekn = ik[(int64_t)(c0 >> 1) * a.k.H], evn = iv[(int64_t)(c0 >> 1) * a.k.H];
+  for (int t = c0; t < nt; ++t) {
     pa_arrived();
     const int b = t & 1, ek = ekn, ev = evn;
     if (t + 1 < nt) {
@@ -634,17 +677,18 @@ VH_DEV void pa_mm_dq_impl(const PaArgs& a, int id, PaHalves lds) {
       for (int db = 0; db < DB; ++db) pa_mma(fk.cols(b, db, u), f, acc[db]);
     }
   }
-  if (!live) return;
-  pa_store<DB>(a.dq + tok * a.dq_t + h * a.dq_h, a.dq_vec, a.D, acc,
-               [&](float v) { return pa_ldexp(v * a.scale, top - PA_E - g); });
+  if (!live || mine <= c0) return;
+  const bool whole = a.chunks == 1;
+  pa_store<DB>(whole ? a.dq + tok * a.dq_t + h * a.dq_h : a.fold + pa_fold_at(a, part, tok, h), whole ? a.dq_vec : 1,
+               whole ? a.D : DP, acc, [&](float v) { return pa_ldexp(v * a.scale, top - PA_E - g); });
 }
 
 // dk and dv: a workgroup per block of 32 NW keys, key head and part of its query heads,
 // 32 keys a wave, over the queries that see them, 32 at a time; Q and dO are read by
 // rows for S and dO V^T and by columns for dV and dK. Its accumulators and resident rows
 // leave no registers for a second step's S: what overlaps is the exp of S with dO V^T and
-// dS with dV. Where the blocks are few the query heads are divided over a.parts workgroups,
-// whose sums pa_join adds in order. HALVES 2: a workgroup forms one half of dk's and dv's
+// dS with dV. Where the blocks are few the steps of all its query heads are divided over
+// a.parts workgroups, whose sums pa_join adds in order. HALVES 2: a workgroup forms one half of dk's and dv's
 // elements, all of which are too many registers past 128.
 template <int DP, int NW, int HALVES>
 VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, PaHalves lds) {
@@ -655,16 +699,15 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, PaHalves lds) {
   if (id >= a.head->nblocks * H) return;
   // Keys' cost falls along a causal sequence where queries' rises: its blocks from the end.
   if (a.causal) sp.row0 = (sp.len - 1) / a.block_rows * a.block_rows - sp.row0;
-  const int G = a.q.H / a.k.H, per = (G + a.parts - 1) / a.parts;
-  const int part = id % H % a.parts, hk = id % H / a.parts;
-  const int h0 = hk * G + part * per, h1 = min(h0 + per, (hk + 1) * G);
+  const int G = a.q.H / a.k.H, part = id % H % a.parts, hk = id % H / a.parts;
   const int lane = threadIdx.x & 63, w = pa_wave(), hf = lane >> 5;
   const PaStream &sk = a.stream[0], &sv = a.stream[1], &sq = a.stream[2], &sg = a.stream[3];
   const int t0 = a.causal ? sp.row0 >> 5 : 0, t1 = (sp.len + 31) >> 5;
   const PaStage<DP> fq(lq), fg(lg);
   const int r0 = sp.row0 + 32 * w, j = r0 + (lane & 31);
   auto stat = [&](int b, int i) { return *(const __attribute__((address_space(3))) pa_f4*)(lst + b * 128 + 2 * i); };
-  const int nt = t1 - t0, steps = nt * (h1 - h0);
+  const int nt = t1 - t0, s0 = (int)((int64_t)nt * G * part / a.parts);
+  const int steps = (int)((int64_t)nt * G * (part + 1) / a.parts) - s0;
   struct At {  // a step's head and 32 queries
     int h, t;
     VH_DEV void next(int t0, int t1) {
@@ -681,7 +724,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, PaHalves lds) {
     pa_copy<NW, 2 * SUB>(sg.n + at, lg + st * SUB);
     if (threadIdx.x < 16) pa_copy16(a.stat + tile(x) * 128 + (x.t & 1) * 64 + threadIdx.x * 4, lst + st * 128);
   };
-  At now{h0, t0}, ahead{h0, t0};  // ahead: the last step staged
+  At now{hk * G + s0 / nt, t0 + s0 % nt}, ahead = now;  // ahead: the last step staged
   if (steps > 0) stage(ahead, 0);
   PaFrag k[KS], v[KS];
   const int ek = pa_own<DP>(a.k, sp, a.D, j, hk, k), ev = pa_own<DP>(a.v, sp, a.D, j, hk, v);
@@ -694,7 +737,7 @@ VH_DEV void pa_mm_dkdv_impl(const PaArgs& a, int item, PaHalves lds) {
   const bool slow_q = rq.any_slow(topq), slow_g = rg.any_slow(topg);
   if (slow_q || slow_g) {
     pa_arrived();
-    if (half == 0) pa_rows<2>(a, hk, sp, (PaLds)lq, h0, h1, part);
+    if (half == 0) pa_rows<2>(a, hk, sp, (PaLds)lq, hk * G + G * part / a.parts, hk * G + G * (part + 1) / a.parts, part);
     return;
   }
   const float cs = a.scale * PA_LOG2E;
@@ -778,13 +821,33 @@ VH_DEV void pa_mm_bwd_impl(const PaArgs& a, PaHalves lds) {
   else pa_mm_dq_impl<DP, NW>(a, blockIdx.x - n, lds);
 }
 
-// dk and dv of each token in a sequence: the parts' sums, in order. Grid: (tiles,
-// key heads, dk and dv).
+// dk, dv and dq of each token in a sequence: the parts' or chunks' sums, in order. Grid:
+// (tiles, heads, dk and dv and dq).
 template <int DP>
 VH_DEV void pa_join_impl(const PaArgs& a) {
   if ((int)blockIdx.x >= a.head->ntiles) return;
   const PaSpan sp = a.tiles[blockIdx.x];
   const int hk = blockIdx.y, z = blockIdx.z, rows = min(64, sp.len - sp.row0);
+  if (z == 2) {
+    if (a.chunks == 1) return;
+    const int per = pa_chunk(a, sp, sp.row0 / a.block_rows * a.block_rows);
+    for (int u = threadIdx.x; u < rows * (DP / 4); u += 256) {
+      const int row = sp.row0 + u / (DP / 4), d = u % (DP / 4) * 4, used = (pa_steps(a, sp, row & ~31, 32) + per - 1) / per;
+      const int64_t tok = (int64_t)sp.start + row;
+      pa_f4 s = *reinterpret_cast<const pa_f4*>(a.fold + pa_fold_at(a, 0, tok, hk) + d);
+      for (int c = 1; c < used; ++c) s += *reinterpret_cast<const pa_f4*>(a.fold + pa_fold_at(a, c, tok, hk) + d);
+      float* q = a.dq + tok * a.dq_t + hk * a.dq_h + d;
+      if (a.dq_vec) {
+        if (d < a.D) *reinterpret_cast<pa_f4*>(q) = s;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < a.D) q[e] = s[e];
+      }
+    }
+    return;
+  }
+  if (a.parts == 1 || hk >= a.k.H) return;
   float* out = z ? a.dv : a.dk;
   const int64_t ot = z ? a.dv_t : a.dk_t, oh = z ? a.dv_h : a.dk_h, step = (int64_t)2 * a.T * a.k.H * DP;
   for (int u = threadIdx.x; u < rows * (DP / 4); u += 256) {

@@ -125,18 +125,22 @@ constexpr int64_t kPaTogether = 1024;
 // The kernels' head sizes.
 int pa_padded(int64_t D) { return D <= 32 ? 32 : D <= 128 ? (int)cdiv(D, 16) * 16 : (int)cdiv(D, 64) * 64; }
 
-// Workgroups that share a key head's query heads in dk and dv: as many as bring the blocks
-// to kPaJoinBlocks, where a block's first keys meet every query after them. [8192] tokens, 16
-// query heads on 2 of 128: 128 workgroups 7.2 ms, 1024 of an eighth each 2.2.
-constexpr int64_t kPaJoinBlocks = 1024;
-int pa_parts(int64_t T, int64_t Hq, int64_t Hk) {
-  const int64_t G = Hq / Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk)));
-  return (int)cdiv(G, per);
+// Where rows are few, several workgroups take a block: its queries in dk and dv, its keys in
+// the forward and dq. As many as bring the workgroups to kPaSplitBlocks, with four steps of
+// 32 each at the sequences' mean length.
+constexpr int64_t kPaJoinBlocks = 1024, kPaFoldBlocks = 512;
+int64_t pa_mean_steps(int64_t T, int64_t n) { return cdiv(T, 32 * n); }
+int pa_parts(int64_t T, int64_t n, int64_t Hq, int64_t Hk) {
+  const int64_t G = Hq / Hk;
+  return (int)std::clamp<int64_t>(cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk), 1, std::clamp<int64_t>(pa_mean_steps(T, n) * G / 4, 1, 16));
+}
+int pa_chunks(int64_t T, int64_t n, int64_t Hq) {
+  return (int)std::clamp<int64_t>(cdiv(kPaFoldBlocks, cdiv(T, 128) * Hq), 1, std::clamp<int64_t>(pa_mean_steps(T, n) / 4, 1, 8));
 }
 
 // The workspace, in the order its parts are laid out. Streams: k, v, q, dout.
 struct PaScratch {
-  size_t head, tiles, blocks, delta, stat, join, n[4], info[4], total;
+  size_t head, tiles, blocks, delta, stat, join, fold, fold_ml, n[4], info[4], total;
   PaScratch(int64_t T, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, bool backward) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -150,8 +154,10 @@ struct PaScratch {
     blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, seqs, kPaBlockRows));
     delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
     stat = take(backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
-    const int parts = pa_parts(T, Hq, Hk);
+    const int parts = pa_parts(T, seqs, Hq, Hk), chunks = pa_chunks(T, seqs, Hq);
     join = take(backward && parts > 1 ? sizeof(float) * 2 * (size_t)(parts * T * Hk * pa_padded(D)) : 0);
+    fold = take(chunks > 1 ? sizeof(float) * (size_t)(chunks * T * Hq * pa_padded(D)) : 0);
+    fold_ml = take(chunks > 1 && !backward ? 2 * sizeof(float) * (size_t)(chunks * T * Hq) : 0);
     for (int i = 0; i < 4; ++i) {
       const size_t tiles_h = backward || i < 2 ? units * (size_t)(i < 2 ? Hk : Hq) : 0;
       n[i] = take(tiles_h * 256 * (size_t)pa_padded(D));
@@ -218,7 +224,10 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
   a.delta = reinterpret_cast<float*>(p + l.delta);
   a.stat = reinterpret_cast<float*>(p + l.stat);
   a.join = reinterpret_cast<float*>(p + l.join);
-  a.parts = backward ? pa_parts(c->q.T, c->q.H, c->k.H) : 1;
+  a.fold = reinterpret_cast<float*>(p + l.fold);
+  a.fold_ml = reinterpret_cast<float*>(p + l.fold_ml);
+  a.parts = backward ? pa_parts(a.T, a.n, c->q.H, c->k.H) : 1;
+  a.chunks = pa_chunks(a.T, a.n, c->q.H);
   a.grad = -1;
   const PaTensor t[4] = {a.k, a.v, a.q, a.g};
   const int streams = backward ? 4 : 2;
@@ -555,7 +564,9 @@ int vh_packed_attention_fwd(const float* q, const vh_layout* ql, const float* k,
   CallScratch sc;
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   VH_TRY(pa_prepare(&c, lay, sc.p, false, s));
-  return launch("vh_pa_fwd_" + std::to_string(a.DP), a.max_blocks * c.q.H, 1, 1, 256, s, a);
+  const std::string dp = std::to_string(a.DP);
+  VH_TRY(launch("vh_pa_fwd_" + dp, a.max_blocks * c.q.H * a.chunks, 1, 1, 256, s, a));
+  return a.chunks > 1 ? launch("vh_pa_fold_" + dp, a.max_tiles, c.q.H, 1, 256, s, a) : VH_OK;
 }
 
 int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k, const vh_layout* kl, const float* v,
@@ -595,12 +606,13 @@ int vh_packed_attention_bwd(const float* q, const vh_layout* ql, const float* k,
   VH_TRY(sc.get(s, scratch, scratch_bytes, lay.total));
   VH_TRY(pa_prepare(&c, lay, sc.p, true, s));
   const std::string dp = std::to_string(a.DP);
-  const int64_t dkdv = a.max_blocks * c.k.H * a.parts * (a.DP > 128 ? 2 : 1), dqs = a.max_blocks * c.q.H;
+  const int64_t dkdv = a.max_blocks * c.k.H * a.parts * (a.DP > 128 ? 2 : 1), dqs = a.max_blocks * c.q.H * a.chunks;
   // Few workgroups: both in one launch (pa_mm_bwd_impl).
   const bool together = a.DP <= 128 && dkdv + dqs <= kPaTogether;
   VH_TRY(launch((together ? "vh_pa_bwd_" : "vh_pa_dkdv_") + dp, together ? dkdv + dqs : dkdv, 1, 1, 256, s, a));
-  if (a.parts > 1) VH_TRY(launch("vh_pa_join_" + dp, a.max_tiles, c.k.H, 2, 256, s, a));
-  return together ? VH_OK : launch("vh_pa_dq_" + dp, dqs, 1, 1, 256, s, a);
+  if (!together) VH_TRY(launch("vh_pa_dq_" + dp, dqs, 1, 1, 256, s, a));
+  if (a.chunks > 1) return launch("vh_pa_join_" + dp, a.max_tiles, c.q.H, 3, 256, s, a);
+  return a.parts > 1 ? launch("vh_pa_join_" + dp, a.max_tiles, c.k.H, 2, 256, s, a) : VH_OK;
 }
 
 size_t vh_linear_cross_entropy_scratch_bytes(int64_t R, int64_t D, int64_t V, int backward) {

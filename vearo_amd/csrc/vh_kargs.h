@@ -481,7 +481,10 @@ struct PaArgs {
   PaStream stream[4];      // k, v, q, g (forward: the first two)
   int32_t grad;            // the gradient's stream (the prepare launch forms delta with it), or -1
   int32_t out_vec, dq_vec, dk_vec, dv_vec;  // rows may be written as 16-byte units
-  int32_t parts;           // workgroups that divide a key head's query heads (dk and dv)
+  int32_t parts;           // workgroups that divide a block's queries of all heads (dk and dv)
+  int32_t chunks;          // workgroups that divide a block's keys (forward, dq), where it has as many
+  float* fold;             // chunks > 1: [chunks][T][Hq][D padded] rows of o or sums of dq
+  float* fold_ml;          // and the forward's [chunks][Hq][T][2] max and sum of exp
   float* join;             // parts > 1: [parts][dk, dv][T][Hk][D padded] sums
   float* stat;             // [tiles][Hq][2][32 log2-lse - 11, 32 delta]
   float* out;              // forward
