@@ -363,11 +363,11 @@ class Graph:
         self.st.close()
 
 
-@pytest.mark.parametrize("D", [64, 160])
-def test_captured_and_replayed(vh, D):
-    lens = [200, 60]
+@pytest.mark.parametrize("D,lens,second", [(64, [200, 60], [60, 130]), (160, [200, 60], [60, 130]), (64, [900, 100], [330, 650]),
+                                           (128, [900, 100], [330, 650])])
+def test_captured_and_replayed(vh, D, lens, second):
     a = [inputs(lens, 2, 1, D, s) for s in (1, 2)]
-    starts = [R.starts_of(lens), R.starts_of([60, 130])]  # the second batch's sequences are others
+    starts = [R.starts_of(lens), R.starts_of(second)]  # the second batch's sequences are others
     want = [R.Attention(vh, *x, s, 0.1, True).run() for x, s in zip(a, starts)]
     c = R.Attention(vh, *a[0], starts[0], 0.1, True)
     nb = [vh.lib.vh_packed_attention_scratch_bytes(*c.sizes, b) for b in (0, 1)]

@@ -125,17 +125,26 @@ constexpr int64_t kPaTogether = 1024;
 // The kernels' head sizes.
 int pa_padded(int64_t D) { return D <= 32 ? 32 : D <= 128 ? (int)cdiv(D, 16) * 16 : (int)cdiv(D, 64) * 64; }
 
-// Where rows are few, several workgroups take a block: its queries in dk and dv, its keys in
-// the forward and dq. As many as bring the workgroups to kPaSplitBlocks, with four steps of
-// 32 each at the sequences' mean length.
+// Where rows are few, several workgroups take a block: its keys in the forward and dq, its
+// queries in dk and dv. As many as bring the workgroups to kPaFoldBlocks, with eight steps of
+// 32 each at the sequences' mean length (6646 tokens in 3 sequences, 3 heads of 128, forward:
+// 222 us undivided, 128 with 512 workgroups, 140 with 256; of four steps, 1767 tokens in 3, 12
+// on 4 heads of 112, forward and backward: 238 us, of eight 209). In dk and dv, whose first
+// keys meet every query after them, the query heads of a key head alone go up to
+// kPaJoinBlocks: 8192 tokens, 16 on 2 heads of 128, 128 workgroups 7.2 ms, 1024 2.2; 8192
+// tokens, 16 on 4 of 40, forward and backward, 512 1.82 ms, 1024 1.60.
+// Where a CU holds one workgroup (dk and dv from 80 elements on, dq from 112) half of
+// kPaFoldBlocks: 13100 tokens in 26, 3 on 1 heads of 112, 291 -> 265 us.
 constexpr int64_t kPaJoinBlocks = 1024, kPaFoldBlocks = 512;
 int64_t pa_mean_steps(int64_t T, int64_t n) { return cdiv(T, 32 * n); }
-int pa_parts(int64_t T, int64_t n, int64_t Hq, int64_t Hk) {
-  const int64_t G = Hq / Hk;
-  return (int)std::clamp<int64_t>(cdiv(kPaJoinBlocks, cdiv(T, 128) * Hk), 1, std::clamp<int64_t>(pa_mean_steps(T, n) * G / 4, 1, 16));
+int pa_parts(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D) {
+  const int64_t G = Hq / Hk, blocks = cdiv(T, 128) * Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, blocks)));
+  const int64_t want = pa_padded(D) >= 80 ? kPaFoldBlocks / 2 : kPaFoldBlocks;
+  return (int)std::max(cdiv(G, per), std::min<int64_t>({cdiv(want, blocks), pa_mean_steps(T, n) * G / 8, 16}));
 }
-int pa_chunks(int64_t T, int64_t n, int64_t Hq) {
-  return (int)std::clamp<int64_t>(cdiv(kPaFoldBlocks, cdiv(T, 128) * Hq), 1, std::clamp<int64_t>(pa_mean_steps(T, n) / 4, 1, 8));
+int pa_chunks(int64_t T, int64_t n, int64_t Hq, int64_t D, bool backward) {
+  const int64_t want = backward && pa_padded(D) >= 112 ? kPaFoldBlocks / 2 : kPaFoldBlocks;
+  return (int)std::clamp<int64_t>(cdiv(want, cdiv(T, 128) * Hq), 1, std::clamp<int64_t>(pa_mean_steps(T, n) / 8, 1, 8));
 }
 
 // The workspace, in the order its parts are laid out. Streams: k, v, q, dout.
@@ -154,7 +163,7 @@ struct PaScratch {
     blocks = take(sizeof(PaSpan) * (size_t)pa_units(T, seqs, kPaBlockRows));
     delta = take(backward ? sizeof(float) * (size_t)(Hq * T) : 0);
     stat = take(backward ? sizeof(float) * 128 * units * (size_t)Hq : 0);
-    const int parts = pa_parts(T, seqs, Hq, Hk), chunks = pa_chunks(T, seqs, Hq);
+    const int parts = pa_parts(T, seqs, Hq, Hk, D), chunks = pa_chunks(T, seqs, Hq, D, backward);
     join = take(backward && parts > 1 ? sizeof(float) * 2 * (size_t)(parts * T * Hk * pa_padded(D)) : 0);
     fold = take(chunks > 1 ? sizeof(float) * (size_t)(chunks * T * Hq * pa_padded(D)) : 0);
     fold_ml = take(chunks > 1 && !backward ? 2 * sizeof(float) * (size_t)(chunks * T * Hq) : 0);
@@ -226,8 +235,8 @@ int pa_prepare(PaCall* c, const PaScratch& l, void* base, bool backward, hipStre
   a.join = reinterpret_cast<float*>(p + l.join);
   a.fold = reinterpret_cast<float*>(p + l.fold);
   a.fold_ml = reinterpret_cast<float*>(p + l.fold_ml);
-  a.parts = backward ? pa_parts(a.T, a.n, c->q.H, c->k.H) : 1;
-  a.chunks = pa_chunks(a.T, a.n, c->q.H);
+  a.parts = backward ? pa_parts(a.T, a.n, c->q.H, c->k.H, a.D) : 1;
+  a.chunks = pa_chunks(a.T, a.n, c->q.H, a.D, backward);
   a.grad = -1;
   const PaTensor t[4] = {a.k, a.v, a.q, a.g};
   const int streams = backward ? 4 : 2;
