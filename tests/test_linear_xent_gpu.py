@@ -99,6 +99,14 @@ def test_several_pieces(vh):
     Xent(vh, 700, 8, V, 0.3).check()
 
 
+def test_last_piece_with_more_sums(vh):
+    """4352 rows of 512 whole tiles and 100 in five sums, then 3948 of 512 and 64 in eight: the larger lot fits the scratch."""
+    c = Xent(vh, 8300, 4608, 2560, 0.1, scale=0.02)
+    val, tol = R.linear_xent(c.x, c.w, c.t, c.ignore, c.go)
+    c.call("fwd_bwd")
+    R.check(c.results(), val, tol, ["loss", "dx", "dw"])
+
+
 @pytest.mark.parametrize("ignore", [-100.0, 3.0, math.nan])
 def test_ignored(vh, ignore):
     t = np.array([3, 1, 4, 1, 5, 3, 2, 6, 3, 5], np.float32)

@@ -229,7 +229,8 @@ def test_rows_of_very_different_size(vh, name, spread, causal):
 
 
 @pytest.mark.parametrize("lens,Hq,Hk,D", [([700], 8, 1, 32), ([300], 6, 2, 64), ([40] * 100, 8, 4, 128), ([150], 4, 1, 160),
-                                          ([200], 2, 1, 256)])
+                                          ([200], 2, 1, 256),
+                                          ([700], 1, 1, 64), ([1100, 40], 2, 2, 128)])
 def test_rows_of_very_different_size_in_every_launch(vh, lens, Hq, Hk, D):
     """The row forms beside the matrix kernels: query heads in parts, dq with dk and dv, each alone, elements in halves."""
     for n in range(4):

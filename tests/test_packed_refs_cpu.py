@@ -219,6 +219,7 @@ def test_scratch_sizes():
     assert L.vh_packed_attention_scratch_bytes(0, 1, 4, 2, 64, 1) == 0
     assert L.vh_packed_attention_scratch_bytes(16384, 8, 12, 4, 64, 1) >= 4 * 12 * 16384
     assert L.vh_qk_norm_rope_bwd_scratch_bytes(0, 64) == 0 < L.vh_qk_norm_rope_bwd_scratch_bytes(1, 1)
+    assert L.vh_packed_attention_scratch_bytes(100, 1, 2, 4, 64, 1) > 0  # (head counts that a call refuses)
     # A gradient's pieces: three blocks of 683 MiB, and no less than 256 rows of logits. A forward: none.
     assert L.vh_linear_cross_entropy_scratch_bytes(65536, 768, 50257, 1) < 4 * 65536 * 50257 // 4
     assert L.vh_linear_cross_entropy_scratch_bytes(1024, 8, 4000000, 1) >= 4 * 256 * 4000000

@@ -138,7 +138,7 @@ int pa_padded(int64_t D) { return D <= 32 ? 32 : D <= 128 ? (int)cdiv(D, 16) * 1
 constexpr int64_t kPaJoinBlocks = 1024, kPaFoldBlocks = 512;
 int64_t pa_mean_steps(int64_t T, int64_t n) { return cdiv(T, 32 * n); }
 int pa_parts(int64_t T, int64_t n, int64_t Hq, int64_t Hk, int64_t D) {
-  const int64_t G = Hq / Hk, blocks = cdiv(T, 128) * Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, blocks)));
+  const int64_t G = std::max<int64_t>(Hq / Hk, 1), blocks = cdiv(T, 128) * Hk, per = cdiv(G, std::min(G, cdiv(kPaJoinBlocks, blocks)));
   const int64_t want = pa_padded(D) >= 80 ? kPaFoldBlocks / 2 : kPaFoldBlocks;
   return (int)std::max(cdiv(G, per), std::min<int64_t>({cdiv(want, blocks), pa_mean_steps(T, n) * G / 8, 16}));
 }
@@ -316,8 +316,10 @@ struct LxScratch {
     const int64_t rows = lx_rows(R, D, V, backward);
     const bool grad = backward && lx_grad_by_parts(R, D, V);
     const size_t vb = (size_t)cdiv(V, 32), rb = (size_t)cdiv(rows, 256), db = (size_t)cdiv(D, 32);
-    // (The products' sums lie where z did.)
-    const size_t sums = grad ? std::max(LxTiles(rows, D, (int64_t)vb * 2).sums(), LxTiles(V, D, (int64_t)rb * 16).sums()) : 0;
+    // The products' sums lie where z did. (The last piece's may be more: other tiles are divided.)
+    size_t sums = 0;
+    for (int64_t m : {rows, R - (cdiv(R, rows) - 1) * rows})
+      if (grad) sums = std::max({sums, LxTiles(m, D, (int64_t)vb * 2).sums(), LxTiles(V, D, cdiv(m, 256) * 16).sums()});
     z = take(std::max(parts && !backward ? 0 : sizeof(float) * (size_t)(rows * lx_ld(V)), sums));
     top = take(grad ? 2 * sizeof(uint32_t) * (size_t)D : 0);  // column maxima of w, of x
     re = take(grad ? sizeof(int32_t) * 256 * rb : 0);
