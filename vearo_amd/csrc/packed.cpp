@@ -133,7 +133,8 @@ int pa_padded(int64_t D) { return D <= 32 ? 32 : D <= 128 ? (int)cdiv(D, 16) * 1
 // keys meet every query after them, the query heads of a key head alone go up to
 // kPaJoinBlocks: 8192 tokens, 16 on 2 heads of 128, 128 workgroups 7.2 ms, 1024 2.2; 8192
 // tokens, 16 on 4 of 40, forward and backward, 512 1.82 ms, 1024 1.60.
-// Where a CU holds one workgroup (dk and dv from 80 elements on, dq from 112) half of
+// Where a CU holds one workgroup (dk and dv from 96 elements on, dq from 112), and for dk and
+// dv of 80 (11274 tokens in 5, 2 heads: 562 us with 512, 544 with 256), half of
 // kPaFoldBlocks: 13100 tokens in 26, 3 on 1 heads of 112, 291 -> 265 us.
 constexpr int64_t kPaJoinBlocks = 1024, kPaFoldBlocks = 512;
 int64_t pa_mean_steps(int64_t T, int64_t n) { return cdiv(T, 32 * n); }
